@@ -104,6 +104,46 @@ struct UnitRegs {
   u32x4 v[D / 16];     // [dim tile]
 };
 
+// 16 bytes of the cache.  ONCE (a kernel template argument: with both forms behind a run-time branch
+// the compiler merges the two arms and the hint is lost): nothing will read them again in this launch
+// (one group of query rows per sequence and KV head), so they are fetched non-temporally and leave the caches to what is
+// re-used; the decode step runs 10 % faster for it (186 -> 169 us).  With several row groups
+// (prefill) the later ones find K / V in L2 and the plain load is the faster one (778 vs 623 TFLOP/s).
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load_kv16(const uint16_t* p) {
+  if (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return *reinterpret_cast<const u32x4*>(p);
+}
+
+// Issue the 16-byte loads of one 32-token unit.  ids: pool block ids of the
+// unit's two blocks (wave-uniform).
+template <int D, bool ONCE>
+__device__ __forceinline__ void load_unit_k(UnitRegs<D>& r, const PagedAttnParams& p, int kvh, int idA, int idB, int n, int g) {
+  // K: lane (n, g) supplies token 8*(n/4) + 4*tile + n%4 of the unit, i.e. token slot
+  // n % 8 of slab tile `tile` in block A (n < 8) or B; dims 32*kk + 8g .. +8 are dim
+  // chunk 4*kk + g.  A 16-lane quarter (fixed g) reads 128 contiguous bytes per block.
+  const int64_t offA = (int64_t)idA * p.k_bs, offB = (int64_t)idB * p.k_bs;  // wave-uniform products
+  const uint16_t* kp = p.kpool + ((n >= 8) ? offB : offA) + (int64_t)kvh * p.k_hs + g * 64 + (n & 7) * 8;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) r.k[t][kk] = load_kv16<ONCE>(kp + t * (D * 8) + kk * 256);
+}
+template <int D, bool ONCE>
+__device__ __forceinline__ void load_unit_v(UnitRegs<D>& r, const PagedAttnParams& p, int kvh, int idA, int idB, int n, int g) {
+  // V: lane (n, g) supplies dim 16j + n, tokens 8g..8g+7 of the unit: token half g & 1
+  // of block A (g < 2) or B.  A 16-lane quarter reads 256 contiguous bytes.
+  const int64_t voffA = (int64_t)idA * p.v_bs, voffB = (int64_t)idB * p.v_bs;
+  const uint16_t* vp = p.vpool + ((g >= 2) ? voffB : voffA) + (int64_t)kvh * p.v_hs + ((g & 1) * 16 + n) * 8;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) r.v[j] = load_kv16<ONCE>(vp + j * 256);
+}
+template <int D, bool ONCE>
+__device__ __forceinline__ void load_unit(UnitRegs<D>& r, const PagedAttnParams& p, int kvh, int idA, int idB, int n, int g) {
+  load_unit_k<D, ONCE>(r, p, kvh, idA, idB, n, g);
+  load_unit_v<D, ONCE>(r, p, kvh, idA, idB, n, g);
+}
+
 template <int D, int NQT>
 struct RowState {
   f32x4 o[NQT][D / 16];  // O^T accumulators: dims 16j + 4g + i, query row n

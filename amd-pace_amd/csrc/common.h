@@ -31,9 +31,11 @@ void set_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
     }                                                                             \
   } while (0)
 
-// f32_ok: the entry point also takes pools of fp32 rows (elem_bytes 4); otherwise such a pool is refused.
-int check_pool(const pace_kv_pool_t* pool, const char* who, bool f32_ok = false);
+// any_elem: the entry point also takes pools of fp32 rows (elem_bytes 4) and of 4-bit rows (PACE_KV_ELEM_Q4); otherwise
+// such a pool is refused.
+int check_pool(const pace_kv_pool_t* pool, const char* who, bool any_elem = false);
 inline bool pool_is_f32(const pace_kv_pool_t* pool) { return pool->elem_bytes == 4; }
+inline bool pool_is_q4(const pace_kv_pool_t* pool) { return pool->elem_bytes == PACE_KV_ELEM_Q4; }
 int compute_units();  // of the current device
 
 // Dense bf16 attention on the matrix cores (dense_attn_mfma.hip); false = shape not handled, nothing launched.
@@ -44,6 +46,11 @@ bool launch_dense_mfma(const void* q, const void* k, const void* v, void* out, i
 size_t dense_mfma_workspace_bytes(int S, int H, int mB, int mN, int mS, bool has_mask);
 // Attention over a pool of fp32 rows (dense_attn.hip); pool and args are already checked.
 int launch_paged_f32(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* args, const char* who, hipStream_t stream);
+
+// Attention over a pool of 4-bit rows, or through a window (walk_attn.hip); pool and args are already checked.
+int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* args, const char* who, hipStream_t stream);
+int walk_kernel_name(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* args, char* out, size_t cap);
+size_t walk_workspace_bytes(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* args);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -1,7 +1,7 @@
 // Pool data movement for gfx950: append by slot, block-table gather, block copy.
 // All three are pure byte movers bounded by HBM bandwidth; every global access
 // is a 16-byte lane access, coalesced over rows of the token-major side.
-#include "common.h"
+#include "kv_ops.h"
 #include "rope.h"
 
 namespace pace_kv {
@@ -11,17 +11,6 @@ namespace pace_kv {
 // of V.  The K chunk stays one 16-byte store; the V chunk is written token-minor, so
 // its eight values land 16 bytes apart (one per dim) at the token's column.
 // ---------------------------------------------------------------------------------
-// Where the tokens go: either an explicit slot id per token, or "position
-// seq_lens[b] + pos_offset + t of sequence b" resolved through the block table.
-struct AppendDest {
-  const int64_t* slots;
-  const int32_t* table;
-  const int32_t* seq_lens;
-  int32_t table_stride;
-  int32_t pos_offset;
-  const int32_t* offset_dev;  // optional: one more offset, read on the device (a counter a captured graph advances)
-};
-
 template <int D, bool PAGED>
 __global__ __launch_bounds__(256) void kv_append_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
                                                         const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh,
@@ -202,40 +191,6 @@ __global__ __launch_bounds__(256) void kv_append_block_kernel(pace_kv_pool_t poo
 // A workgroup past the end of its sequence leaves at once; the packed form launches none (its grid is
 // built from cu_seqlens).
 // ---------------------------------------------------------------------------------
-struct GatherOut {
-  uint16_t* k;
-  uint16_t* v;
-  const int32_t* cu_seqlens;  // packed form only
-  int64_t stride_b;           // dense: elements between sequences
-  int64_t stride_h;           // elements between output heads
-  int64_t stride_t;           // elements between token rows
-  int32_t out_len;            // dense: rows per sequence; packed: unused
-  int32_t zero_fill;          // dense: write zeros to rows in [len, out_len)
-  int32_t batch;              // packed: sequences (cu_seqlens has batch + 1 entries)
-  int32_t total_rows;         // packed: rows of the outputs
-  int32_t dense_rows;         // packed grid (one workgroup per block that exists), rows written in the dense layout
-};
-
-// Packed grid: which (sequence, head, logical block) workgroup `entry` stands for.
-// One grid entry per (logical block that can exist, KV head): sequence b owns the block entries
-// [cu[b] / 16 + b, cu[b+1] / 16 + b + 1) -- at least ceil(len_b / 16) of them, disjoint, in order -- so a
-// ragged batch launches (almost) no workgroup without rows.  Entries run sequence by sequence, head by
-// head, block by block (the order of the dense grid: with the heads of a block side by side instead the
-// launch measured 6 % slower).  The owner is found by bisection, uniform over the workgroup: scalar loads
-// from a table that stays in the scalar cache.
-__device__ __forceinline__ void packed_entry(const int32_t* __restrict__ cu, int batch, int H, unsigned entry, int& b, int& h, int& j) {
-  int lo = 0, hi = batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if ((int64_t)(cu[mid] / PACE_KV_BLOCK_TOKENS + mid) * H <= (int64_t)entry) lo = mid; else hi = mid;
-  }
-  b = lo;
-  const int first = cu[b] / PACE_KV_BLOCK_TOKENS + b;
-  const int n = cu[b + 1] / PACE_KV_BLOCK_TOKENS + b + 1 - first;  // >= 1
-  const int r = (int)((int64_t)entry - (int64_t)first * H);
-  h = min(r / n, H - 1), j = r % n;
-}
-
 template <int D, bool PACKED>
 __global__ __launch_bounds__(256) void kv_gather_kernel(pace_kv_pool_t pool, const int32_t* __restrict__ table,
                                                         int32_t table_stride, const int32_t* __restrict__ seq_lens,
@@ -425,6 +380,8 @@ static int run_append(const char* who, const pace_kv_pool_t* pool, const void* k
   PACE_REQUIRE(stride_b % per16 == 0 && stride_h % per16 == 0 && stride_t % per16 == 0,
                "%s: input strides must be multiples of %d elements", who, per16);
   hipStream_t s_early = static_cast<hipStream_t>(stream);
+  if (pool_is_q4(pool))
+    return launch_q4_append(who, pool, k_new, v_new, stride_b, stride_h, stride_t, batch, n_tokens, dest, paged, s_early);
   if (pool_is_f32(pool)) {
     const int64_t rows = (int64_t)batch * n_tokens * pool->num_kv_heads;
     PACE_REQUIRE(rows < (int64_t)1 << 31, "%s: too many rows (%lld)", who, (long long)rows);
@@ -514,6 +471,9 @@ static int run_gather(const char* who, const pace_kv_pool_t* pool, const int32_t
                "%s: output strides must be multiples of %d elements and hold a row of head_dim", who, per16);
   const int n_blocks = (rows + PACE_KV_BLOCK_TOKENS - 1) / PACE_KV_BLOCK_TOKENS;
   PACE_REQUIRE(table_stride >= 1, "%s: table_stride %d", who, table_stride);
+  if (pool_is_q4(pool))
+    return launch_q4_gather(who, pool, block_table, table_stride, seq_lens, seq_len_bias, n_rep, out, n_blocks, batch, packed,
+                            static_cast<hipStream_t>(stream));
   // the dense form puts heads and sequences on the grid's y and z axes; the packed form's grid is one-dimensional
   if (!packed) PACE_REQUIRE(batch <= 65535 && pool->num_kv_heads <= 65535, "%s: batch/heads exceed grid limits", who);
   dim3 grid(n_blocks, packed ? 1 : pool->num_kv_heads, packed ? 1 : batch);
@@ -582,9 +542,15 @@ extern "C" int pace_kv_gather_packed(const pace_kv_pool_t* pool, const int32_t* 
                     out, true, stream);
 }
 
-// A slab is copied verbatim, so a pool of fp32 rows is described to the copy kernels in their 2-byte units.
+// A slab is copied verbatim, so pools of other element types are described to the copy kernels in their 2-byte units: one of
+// fp32 rows, and one of 4-bit rows (10 head_dim bytes a slab, that is 16 rows of 5 head_dim / 16 halfwords).
 static pace_kv_pool_t in_halfwords(const pace_kv_pool_t* p) {
   pace_kv_pool_t q = *p;
+  if (pool_is_q4(p)) {
+    q.k_block_stride /= 2, q.k_head_stride /= 2, q.v_block_stride /= 2, q.v_head_stride /= 2;
+    q.head_dim = 5 * p->head_dim / 16;
+    q.elem_bytes = 2;
+  }
   if (pool_is_f32(p)) {
     q.k_block_stride *= 2, q.k_head_stride *= 2, q.v_block_stride *= 2, q.v_head_stride *= 2, q.head_dim *= 2;
     q.elem_bytes = 2;
@@ -596,7 +562,7 @@ extern "C" int pace_kv_copy_blocks(const pace_kv_pool_t* src_in, const pace_kv_p
                                    int32_t n_pairs, void* stream) {
   if (int rc = check_pool(src_in, "pace_kv_copy_blocks(src)", true)) return rc;
   if (int rc = check_pool(dst_in, "pace_kv_copy_blocks(dst)", true)) return rc;
-  PACE_REQUIRE(pool_is_f32(src_in) == pool_is_f32(dst_in), "pace_kv_copy_blocks: src and dst pools differ in element type");
+  PACE_REQUIRE(pool_is_f32(src_in) == pool_is_f32(dst_in) && pool_is_q4(src_in) == pool_is_q4(dst_in), "pace_kv_copy_blocks: src and dst pools differ in element type");
   const pace_kv_pool_t src_h = in_halfwords(src_in), dst_h = in_halfwords(dst_in);
   const pace_kv_pool_t* src = &src_h;
   const pace_kv_pool_t* dst = &dst_h;

@@ -16,46 +16,6 @@
 
 namespace pace_kv {
 
-// 16 bytes of the cache.  ONCE (a kernel template argument: with both forms behind a run-time branch
-// the compiler merges the two arms and the hint is lost): nothing will read them again in this launch
-// (one group of query rows per sequence and KV head), so they are fetched non-temporally and leave the caches to what is
-// re-used; the decode step runs 10 % faster for it (186 -> 169 us).  With several row groups
-// (prefill) the later ones find K / V in L2 and the plain load is the faster one (778 vs 623 TFLOP/s).
-template <bool ONCE>
-__device__ __forceinline__ u32x4 load_kv16(const uint16_t* p) {
-  if (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-  return *reinterpret_cast<const u32x4*>(p);
-}
-
-// Issue the 16-byte loads of one 32-token unit.  ids: pool block ids of the
-// unit's two blocks (wave-uniform).
-template <int D, bool ONCE>
-__device__ __forceinline__ void load_unit_k(UnitRegs<D>& r, const PagedAttnParams& p, int kvh, int idA, int idB, int n, int g) {
-  // K: lane (n, g) supplies token 8*(n/4) + 4*tile + n%4 of the unit, i.e. token slot
-  // n % 8 of slab tile `tile` in block A (n < 8) or B; dims 32*kk + 8g .. +8 are dim
-  // chunk 4*kk + g.  A 16-lane quarter (fixed g) reads 128 contiguous bytes per block.
-  const int64_t offA = (int64_t)idA * p.k_bs, offB = (int64_t)idB * p.k_bs;  // wave-uniform products
-  const uint16_t* kp = p.kpool + ((n >= 8) ? offB : offA) + (int64_t)kvh * p.k_hs + g * 64 + (n & 7) * 8;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int kk = 0; kk < D / 32; ++kk) r.k[t][kk] = load_kv16<ONCE>(kp + t * (D * 8) + kk * 256);
-}
-template <int D, bool ONCE>
-__device__ __forceinline__ void load_unit_v(UnitRegs<D>& r, const PagedAttnParams& p, int kvh, int idA, int idB, int n, int g) {
-  // V: lane (n, g) supplies dim 16j + n, tokens 8g..8g+7 of the unit: token half g & 1
-  // of block A (g < 2) or B.  A 16-lane quarter reads 256 contiguous bytes.
-  const int64_t voffA = (int64_t)idA * p.v_bs, voffB = (int64_t)idB * p.v_bs;
-  const uint16_t* vp = p.vpool + ((g >= 2) ? voffB : voffA) + (int64_t)kvh * p.v_hs + ((g & 1) * 16 + n) * 8;
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j) r.v[j] = load_kv16<ONCE>(vp + j * 256);
-}
-template <int D, bool ONCE>
-__device__ __forceinline__ void load_unit(UnitRegs<D>& r, const PagedAttnParams& p, int kvh, int idA, int idB, int n, int g) {
-  load_unit_k<D, ONCE>(r, p, kvh, idA, idB, n, g);
-  load_unit_v<D, ONCE>(r, p, kvh, idA, idB, n, g);
-}
-
 // The "unit" made of the step's new tokens, read straight from the caller's [T][D] rows
 // (token idx of the unit = new token idx; tokens >= n_new are zero and get masked).
 template <int D, bool ROPE>
@@ -1079,6 +1039,9 @@ static int run_paged_attn(const pace_kv_pool_t* pool, const pace_paged_attn_args
   PACE_REQUIRE(a->q && a->out && a->block_table && a->seq_lens, "%s: NULL q / out / block_table / seq_lens", who);
   PACE_REQUIRE(a->num_q_heads % pool->num_kv_heads == 0, "%s: num_q_heads %d not a multiple of num_kv_heads %d", who,
                a->num_q_heads, pool->num_kv_heads);
+  PACE_REQUIRE(a->window >= 0 && a->sinks >= 0, "%s: negative window (%d) or sinks (%d)", who, a->window, a->sinks);
+  PACE_REQUIRE(a->window > 0 || a->sinks == 0, "%s: sinks (%d) come with a window", who, a->sinks);
+  PACE_REQUIRE(!pool_is_f32(pool) || a->window == 0, "%s: a window over an fp32 pool is not supported", who);
   if (pool_is_f32(pool)) {
     // rows of fp32: the general kernel of the dense operator walks the block table (dense_attn.hip)
     PACE_REQUIRE(!a->rope, "%s: an fp32 pool takes no rotary embedding inside the attention launch", who);
@@ -1129,6 +1092,18 @@ static int run_paged_attn(const pace_kv_pool_t* pool, const pace_paged_attn_args
     PACE_REQUIRE(aligned16(a->k_new) && aligned16(a->v_new) && (a->new_stride_b % 8) == 0 && (a->new_stride_h % 8) == 0 &&
                      (a->new_stride_t % 8) == 0,
                  "%s: k_new / v_new must be 16-byte aligned with strides that are multiples of 8 elements", who);
+  }
+  if (pool_is_q4(pool) || a->window > 0) {
+    // rows of 4 bits, or a window: kernels of their own (walk_attn.hip)
+    PACE_REQUIRE(!a->rope, "%s: no rotary embedding inside the attention launch over a 4-bit pool or through a window", who);
+    PACE_REQUIRE(a->partition_tokens >= 0 && a->partition_tokens % 32 == 0, "%s: partition_tokens %d must be 0 or a multiple of 32", who,
+                 a->partition_tokens);
+    if (g_name_out) return walk_kernel_name(pool, a, g_name_out, g_name_cap);
+    if (!use_static_scratch) {
+      void* unused = nullptr;
+      (void)static_scratch(who, &unused);  // (as below: the look-up belongs to the first call on a device, whichever it is)
+    }
+    return launch_walk(pool, a, who, static_cast<hipStream_t>(stream));
   }
   RopeDev rope_dev = {};
   if (a->rope) {
@@ -1301,6 +1276,22 @@ extern "C" size_t pace_paged_attn_workspace_bytes_for_parts(int32_t batch, int32
   if (batch <= 0 || num_q_heads <= 0 || q_len <= 0 || head_dim <= 0 || max_parts < 1) return 0;
   // rows per KV head are not known here: room for the per-row mask summary whenever the launch could be prefill-sized
   return workspace_need(batch, num_q_heads, q_len, head_dim, max_parts, q_len * num_q_heads);
+}
+
+extern "C" size_t pace_paged_attn_workspace_for(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* args) {
+  if (!pool || !args || args->batch <= 0 || args->num_q_heads <= 0 || args->q_len <= 0 || pool->head_dim <= 0 || pool->num_kv_heads <= 0 ||
+      args->num_q_heads % pool->num_kv_heads)
+    return 0;
+  if (pool_is_q4(pool) || args->window > 0) return walk_workspace_bytes(pool, args);
+  if (pool_is_f32(pool)) {
+    // (what helps a batch that leaves compute units idle: up to 64 workgroups per sequence)
+    const int64_t rows = (int64_t)args->q_len * (args->num_q_heads / pool->num_kv_heads);
+    if ((int64_t)args->batch * pool->num_kv_heads * (rows > 32 ? (rows + 63) / 64 : 1) >= 512) return 0;
+    return (size_t)args->batch * args->num_q_heads * args->q_len * 64 * (pool->head_dim + 4) * sizeof(float);
+  }
+  if (args->work_items) return pace_paged_attn_workspace_bytes_for_parts(args->batch, args->num_q_heads, args->q_len, pool->head_dim, args->max_parts);
+  return pace_paged_attn_workspace_bytes(args->batch, args->num_q_heads, args->q_len, pool->head_dim, args->max_seq_len,
+                                         args->partition_tokens, pool->num_kv_heads);
 }
 
 extern "C" int pace_paged_attn_kernel_name(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* args, char* out,

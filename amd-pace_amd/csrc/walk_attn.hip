@@ -1,0 +1,560 @@
+// Attention over a pool of 4-bit rows, and attention through a window with sinks over a 4-bit or a bf16 pool.
+//
+// The query rows of one KV head are the q_len * n_rep (token, GQA replica) pairs, 16 to a tile, as in attn_core.h, whose
+// operand layouts this file shares: scores of tokens 8 g .. 8 g + 7 of a 32-token unit for query row n sit in lane (n, g),
+// which is where the second product wants the weights.
+//
+// Which tokens: a row at position pos reads t <= pos (or what the mask tensor allows) and, with a window w, only
+// t > pos - w or t < kv_start + sinks.  The units some row of a group reads are two runs -- the sinks' and the window's -- and
+// only they are walked: a step through a window costs the same at any length.
+//
+// 4-bit rows: a value is s * code + m with a step and a middle per token and 32 dims.  Codes become halves by one `and-or`
+// per pair (1024 + code + 8), one packed add and one packed multiply-add, and both products run on halves, which hold
+// the values to 2^-12 (bf16 would keep 2^-9).  Queries are brought into a half's range by a power of two per row, exactly
+// except for components 2^-28 below the row's largest; weights lie in (0, 2^15].
+// 16-bit rows are bf16 products, weights rounded to bf16, as in the kernels without a window.
+#include <algorithm>
+
+#include "attn_core.h"
+#include "kv_ops.h"
+#include "q4.h"
+
+namespace pace_kv {
+
+struct WalkParams : PagedAttnParams {
+  int32_t window, sinks;  // 0: off
+  int32_t part_units;     // 32-token units per workgroup
+};
+
+// The units a group of rows walks: [su0, su0 + n_sink), then [wu0, wu0 + total - n_sink).
+struct Walk {
+  int su0, n_sink, wu0, total, sink_end;
+  __device__ __forceinline__ int unit(int i) const { return i < n_sink ? su0 + i : wu0 + (i - n_sink); }
+};
+
+// s_first, s_last: query tokens of the group's first and last row.
+__device__ __forceinline__ Walk walk_of(const WalkParams& p, int len, int start, int s_first, int s_last) {
+  Walk w;
+  const int end = p.causal ? min(len, len - p.q_len + s_last + 1) : len;
+  int low = start;
+  w.sink_end = start;
+  if (p.window > 0) {
+    low = max(start, len - p.q_len + s_first - p.window + 1);
+    w.sink_end = start + p.sinks;
+  }
+  w.wu0 = low / 32;
+  const int wu1 = end > low ? (end + 31) / 32 : w.wu0;
+  w.su0 = start / 32;
+  w.n_sink = min(w.sink_end, end) > start ? max(min((min(w.sink_end, end) + 31) / 32, w.wu0) - w.su0, 0) : 0;
+  w.total = w.n_sink + wu1 - w.wu0;
+  return w;
+}
+
+__device__ __forceinline__ int walk_len(const WalkParams& p, int b) {
+  return max(p.seq_lens[b] + p.len_bias + (p.len_bias_dev ? *p.len_bias_dev : 0), 0);
+}
+__device__ __forceinline__ int walk_start(const WalkParams& p, int b, int len) { return p.kv_start ? min(max(p.kv_start[b], 0), len) : 0; }
+__device__ __forceinline__ int walk_parts(const WalkParams& p, int total) { return min(max((total + p.part_units - 1) / p.part_units, 1), p.max_parts); }
+
+// ---- one unit of either pool ------------------------------------------------------------------------------------
+template <int N>
+struct Dwords {
+  typedef uint32_t type __attribute__((ext_vector_type(N), aligned(4)));
+};
+template <int N>
+__device__ __forceinline__ void load_dwords(uint32_t (&r)[N], const uint32_t* at) {
+  const typename Dwords<N>::type v = __builtin_nontemporal_load(reinterpret_cast<const typename Dwords<N>::type*>(at));
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = v[i];
+}
+// (scales: sixteen lanes, or four, want the same bytes)
+template <int N>
+__device__ __forceinline__ void load_shared(uint32_t (&r)[N], const uint32_t* at) {
+  const typename Dwords<N>::type v = *reinterpret_cast<const typename Dwords<N>::type*>(at);
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = v[i];
+}
+
+template <int BITS, int D>
+struct WalkUnit;
+
+template <int D>
+struct WalkUnit<16, D> {
+  UnitRegs<D> r;
+  __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int n, int g) { load_unit<D, false>(r, p, kvh, idA, idB, n, g); }
+  __device__ __forceinline__ u32x4 k(int t, int kk) const { return r.k[t][kk]; }
+  __device__ __forceinline__ u32x4 v(int j) const { return r.v[j]; }
+};
+
+template <int D>
+struct WalkUnit<4, D> {
+  using L = Q4<D>;
+  uint32_t kc[2][L::KN][L::KC];  // K codes: [tile][load][dword], step kk = load * KC + dword
+  uint32_t ks[2][L::KN][L::KC];  // K steps and middles of this lane's token
+  uint32_t vc[L::VN][L::VC];     // V codes: dim tile j = load * VC + dword
+  uint32_t vs[L::G][4], vm[L::G][4];  // V steps and middles of this lane's eight tokens, per group of dims
+  __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int n, int g) {
+    const int64_t ka = (int64_t)idA * p.k_bs, kb = (int64_t)idB * p.k_bs, va = (int64_t)idA * p.v_bs, vb = (int64_t)idB * p.v_bs;
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.kpool) + (n >= 8 ? kb : ka) + (int64_t)kvh * p.k_hs);
+    const uint32_t* vp = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.vpool) + (g >= 2 ? vb : va) + (int64_t)kvh * p.v_hs);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < L::KN; ++i) {
+        load_dwords<L::KC>(kc[t][i], kp + L::k_code(t, g, n & 7, i * L::KC));
+        load_shared<L::KC>(ks[t][i], kp + L::k_scale(t, n & 7, i * L::KC));
+      }
+#pragma unroll
+    for (int i = 0; i < L::VN; ++i) load_dwords<L::VC>(vc[i], vp + L::v_code(g & 1, i * L::VC, n));
+#pragma unroll
+    for (int kk = 0; kk < L::G; ++kk) {
+      load_shared<4>(vs[kk], vp + L::v_scale(kk, 8 * (g & 1)) / 2);
+      load_shared<4>(vm[kk], vp + (L::v_scale(kk, 8 * (g & 1)) + 16 * L::G) / 2);
+    }
+  }
+  __device__ __forceinline__ u32x4 k(int t, int kk) const {
+    const f16x2 sm = __builtin_bit_cast(f16x2, ks[t][kk / L::KC][kk % L::KC]);
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r[i] = __builtin_bit_cast(uint32_t, q4_pair(kc[t][kk / L::KC][kk % L::KC], i, f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]}));
+    return r;
+  }
+  __device__ __forceinline__ u32x4 v(int j) const {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r[i] = __builtin_bit_cast(uint32_t, q4_pair(vc[j / L::VC][j % L::VC], i, __builtin_bit_cast(f16x2, vs[j / 2][i]),
+                                                  __builtin_bit_cast(f16x2, vm[j / 2][i])));
+    return r;
+  }
+};
+
+template <int BITS>
+__device__ __forceinline__ f32x4 walk_mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (BITS == 4)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// ---- rows -------------------------------------------------------------------------------------------------------
+template <int D, int NQT>
+struct WalkRows {
+  u32x4 q[NQT][D / 32];
+  f32x4 o[NQT][D / 16];
+  float m[NQT], m_top[NQT], m_neg[NQT], l[NQT];  // see RowState
+  float c[NQT];    // score product -> log2 units
+  float cn[NQT];   // score product -> natural units (with a mask tensor)
+  int limit[NQT];  // last readable token (-1: no such row, or none)
+  int low[NQT];    // with a window: first token of it
+  int64_t mask_off[NQT];
+};
+
+// Weights of halves are kept a factor 2^7 up: with the lazy reference they then reach 2^15, and keep their eleven bits
+// down to 2^-21 of the row's largest.
+template <int BITS>
+constexpr float kWeightShift = BITS == 4 ? 7.f : 0.f;
+
+// Query row -> operand registers; 4-bit pools: as halves, times the power of two that brings the row's largest component to
+// [2^14, 2^15) (returned as its exponent; the four lanes (n, 0..3) of a row agree).
+template <int BITS, int D>
+__device__ __forceinline__ int walk_query(u32x4 (&q)[D / 32]) {
+  if constexpr (BITS == 16) {
+    return 0;
+  } else {
+    float top = 0.f;
+    float x[D / 32][8];
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) {
+      bf16x8_to_f32(q[kk], x[kk]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[kk][e]));
+    }
+    top = fmaxf(top, xor_lanes(top, 16));
+    top = fmaxf(top, xor_lanes(top, 32));
+    const int e = (int)((__float_as_uint(top) >> 23) & 255u);
+    const int up = (e == 0 || e == 255) ? 0 : min(14 - (e - 127), 120);  // (0 and infinity stay what they are)
+    const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        q[kk][i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(x[kk][2 * i] * f), (_Float16)(x[kk][2 * i + 1] * f)});
+    return up;
+  }
+}
+
+// One unit: FULL = every row reads all of its 32 tokens.
+template <int BITS, int D, int NQT, bool HAS_MASK, bool FULL>
+__device__ __forceinline__ void walk_unit(const WalkUnit<BITS, D>& u, WalkRows<D, NQT>& st, int t0, int start, int sink_end, int row_low,
+                                          int row_end, int g, const MaskRegs<NQT>& mregs) {
+#pragma clang fp contract(off)
+  constexpr int KK = D / 32, MT = D / 16;
+  const int base = t0 + 8 * g;  // this lane's first token
+  f32x4 sc[NQT][2];
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) sc[qt][0] = sc[qt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const u32x4 k = u.k(t, kk);
+#pragma unroll
+      for (int qt = 0; qt < NQT; ++qt) sc[qt][t] = walk_mfma<BITS>(k, st.q[qt][kk], sc[qt][t]);
+    }
+  u32x4 pb[NQT];
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s[e] = sc[qt][e >> 2][e & 3];
+      if (HAS_MASK) s[e] = __builtin_fmaf(s[e], st.cn[qt], mregs.a[qt][e]);
+    }
+    if (!FULL) {
+      const int hi = st.limit[qt] - base, lo = start - base, wl = st.low[qt] - base, se = sink_end - base;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e > hi || e < lo || (e < wl && e >= se)) s[e] = kNegInf;  // whatever the token holds
+    }
+    const float c = HAS_MASK ? kLog2e : st.c[qt];
+    const float top = st.m_top[qt];
+    bool above = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) above = above || s[e] > top;
+    if (__any(above)) {  // the reference follows the maximum lazily, as in softmax_and_output
+      const float mx = row_max4(fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))));
+      const float m_old = st.m[qt], m_new = fmaxf(m_old, mx);
+      const float m_use = m_new == kNegInf ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f((m_old - m_use) * c);
+      st.m[qt] = m_new;
+      st.m_top[qt] = m_new + kLazyLog2 / c;
+      st.m_neg[qt] = kWeightShift<BITS> - m_use * c;
+      st.l[qt] *= alpha;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) st.o[qt][j] *= alpha;
+    }
+    float w[8], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, st.m_neg[qt]));
+      sum += w[e];
+    }
+    st.l[qt] += sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (BITS == 4) pb[qt][i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)w[2 * i], (_Float16)w[2 * i + 1]});
+      else pb[qt][i] = pack_bf16x2(w[2 * i], w[2 * i + 1]);
+    }
+  }
+  // Tokens that no row of the wave reads (past the end, between the sinks and the window) may hold anything in a 16-bit pool: their
+  // weight is 0, and 0 times infinity must not be added.  A 4-bit pool holds finite values only.
+  u32x4 keep = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+  if (!FULL && BITS == 16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int t = base + e;
+      if (t < start || t >= row_end || (t < row_low && t >= sink_end)) keep[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    u32x4 v = u.v(j);
+    if (!FULL && BITS == 16) v &= keep;
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) st.o[qt][j] = walk_mfma<BITS>(v, pb[qt], st.o[qt][j]);
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// NW waves split a partition's units among themselves (wave w: units w, w + NW, ...) and merge through LDS.
+// ---------------------------------------------------------------------------------
+template <int BITS, int D, int NQT, bool HAS_MASK, int NW, int OCC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8))) void walk_attn_kernel(const WalkParams p) {
+  constexpr int KK = D / 32, MT = D / 16;
+  __shared__ float merge_buf[(NW / 2) * 16 * NQT * (D + 2)];
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t item = blockIdx.x;  // KV head fastest (one head's K / V stay in one XCD's L2), then partition, row group, sequence
+  const int kvh = (int)(item % (uint32_t)p.num_kv_heads);
+  const uint32_t rest = item / (uint32_t)p.num_kv_heads;
+  const int part = (int)(rest % (uint32_t)p.max_parts);
+  const uint32_t bz = rest / (uint32_t)p.max_parts;
+  const int qg = (int)(bz % (uint32_t)p.n_qgroups), b = (int)(bz / (uint32_t)p.n_qgroups);
+  const int len = walk_len(p, b), start = walk_start(p, b, len);
+  const int S = p.q_len, R = S * p.n_rep;
+  const int r_first = qg * NQT * 16, r_last = min(R, r_first + NQT * 16) - 1;
+  const int s_first = r_first / p.n_rep, s_last = r_last / p.n_rep;
+  const Walk walk = walk_of(p, len, start, s_first, s_last);
+  const int n_parts = walk_parts(p, walk.total);
+  if (part >= n_parts) return;  // uniform over the workgroup
+  const int i_begin = part * p.part_units, i_end = part == n_parts - 1 ? walk.total : min(i_begin + p.part_units, walk.total);
+  const int n_mine = i_end - i_begin > wave ? (i_end - i_begin - wave + NW - 1) / NW : 0;
+
+  // Pool block ids of 32 units of this wave, one per lane; never outside the pool, whatever the table holds.
+  const int32_t* row = p.table + (int64_t)b * p.table_stride;
+  auto fetch_ids = [&](int first) {
+    const int i = i_begin + wave + NW * (first + (lane >> 1));
+    const int at = 2 * walk.unit(i) + (lane & 1);
+    const int id = i < i_end && at < p.table_stride ? row[at] : 0;
+    return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
+  };
+  int ids = fetch_ids(0);
+
+  WalkRows<D, NQT> st;
+  int row_s[NQT], row_h[NQT], min_limit = 0x7fffffff;
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+    const int r = r_first + qt * 16 + n;
+    const bool valid = r < R;
+    const int s = valid ? r / p.n_rep : 0, hq = kvh * p.n_rep + (valid ? r % p.n_rep : 0), pos = len - S + s;
+    row_s[qt] = s, row_h[qt] = hq;
+    st.limit[qt] = valid ? (p.causal ? pos : len - 1) : -1;
+    st.low[qt] = p.window > 0 ? pos - p.window + 1 : 0;
+    if (valid) min_limit = min(min_limit, st.limit[qt]);
+    st.mask_off[qt] = HAS_MASK ? (int64_t)b * p.m_sb + (int64_t)s * p.m_ss : 0;
+    const uint16_t* qp = p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh + (int64_t)s * p.q_ss + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) st.q[qt][kk] = valid ? *reinterpret_cast<const u32x4*>(qp + kk * 32) : u32x4{0u, 0u, 0u, 0u};
+    const int up = walk_query<BITS, D>(st.q[qt]);
+    const float down = __uint_as_float((uint32_t)(127 - up) << 23);
+    st.cn[qt] = p.scale * down;
+    st.c[qt] = fminf(fmaxf(p.scale_log2 * down, 0x1p-126f), 0x1p126f);  // (not 0 or infinite: it multiplies -inf and 0)
+    st.m[qt] = kNegInf, st.m_top[qt] = kNegInf, st.m_neg[qt] = 0.f, st.l[qt] = 0.f;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) st.o[qt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o *= 2) min_limit = min(min_limit, __shfl_xor(min_limit, o, 64));
+  min_limit = __builtin_amdgcn_readfirstlane(min_limit);
+  const int row_low = p.window > 0 ? len - S + s_first - p.window + 1 : 0;  // lowest window start of the group
+  const int max_low = p.window > 0 ? len - S + s_last - p.window + 1 : 0;   // highest
+  const int row_end = p.causal ? min(len, len - S + s_last + 1) : len;
+
+  for (int k = 0; k < n_mine; ++k) {
+    if (k != 0 && (k & 31) == 0) ids = fetch_ids(k);
+    const int t0 = 32 * walk.unit(i_begin + wave + NW * k);
+    MaskRegs<NQT> mregs;
+    if (HAS_MASK) load_mask_regs<NQT>(mregs, p, st.mask_off, t0, g);
+    WalkUnit<BITS, D> u;
+    u.load(p, kvh, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1), n, g);
+    const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
+    if (full) walk_unit<BITS, D, NQT, HAS_MASK, true>(u, st, t0, start, walk.sink_end, row_low, row_end, g, mregs);
+    else walk_unit<BITS, D, NQT, HAS_MASK, false>(u, st, t0, start, walk.sink_end, row_low, row_end, g, mregs);
+  }
+
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+    st.l[qt] += xor_lanes(st.l[qt], 16);
+    st.l[qt] += xor_lanes(st.l[qt], 32);
+    st.m[qt] *= HAS_MASK ? kLog2e : st.c[qt];  // log2 units; -inf stays -inf
+  }
+  // Pairwise merge of the waves' states (fixed order: the same bits from call to call).
+  constexpr int ROW_F = D + 2, SLOT_F = 16 * NQT * ROW_F;
+#pragma unroll
+  for (int stride = 1; stride < NW; stride *= 2) {
+    const int slot = wave / (2 * stride);
+    const bool sender = (wave & (2 * stride - 1)) == stride, receiver = (wave & (2 * stride - 1)) == 0;
+    if (sender) {
+#pragma unroll
+      for (int qt = 0; qt < NQT; ++qt) {
+        float* to = merge_buf + slot * SLOT_F + (qt * 16 + n) * ROW_F;
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to[16 * j + 4 * g + i] = st.o[qt][j][i];
+        if (g == 0) to[D] = st.m[qt], to[D + 1] = st.l[qt];
+      }
+    }
+    __syncthreads();
+    if (receiver) {
+#pragma unroll
+      for (int qt = 0; qt < NQT; ++qt) {
+        const float* from = merge_buf + slot * SLOT_F + (qt * 16 + n) * ROW_F;
+        const float m_b = from[D], l_b = from[D + 1], m_new = fmaxf(st.m[qt], m_b), m_use = m_new == kNegInf ? 0.f : m_new;
+        const float wa = __builtin_amdgcn_exp2f(st.m[qt] - m_use), wb = __builtin_amdgcn_exp2f(m_b - m_use);
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.o[qt][j][i] = st.o[qt][j][i] * wa + from[16 * j + 4 * g + i] * wb;
+        st.l[qt] = st.l[qt] * wa + l_b * wb;
+        st.m[qt] = m_new;
+      }
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+    if (r_first + qt * 16 + n >= R) continue;
+    const float l = st.l[qt];
+    if (p.max_parts == 1) {
+      const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that read nothing is 0; NaN stays NaN
+      uint16_t* op = p.out + (int64_t)b * p.o_sb + (int64_t)row_h[qt] * p.o_sh + (int64_t)row_s[qt] * p.o_ss + 4 * g;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const f32x4 o = st.o[qt][j];
+        *reinterpret_cast<u32x2*>(op + 16 * j) = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+      }
+    } else {
+      const int64_t at = (((int64_t)b * p.num_q_heads + row_h[qt]) * S + row_s[qt]) * p.max_parts + part;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * j + 4 * g) = st.o[qt][j];
+      if (g == 0) *reinterpret_cast<u32x2*>(p.part_ml + 2 * at) = u32x2{__float_as_uint(st.m[qt]), __float_as_uint(l)};
+    }
+  }
+}
+
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partitions of a query row, one wave per row.  A lane fetches the
+// (maximum, sum) pair of one partition, and owns the dims 2 lane, 2 lane + 1 (+ 128).
+template <int D>
+__global__ __launch_bounds__(64) void walk_merge_kernel(const WalkParams p, int32_t rows_per_group) {
+  constexpr int PASSES = (D + 127) / 128;
+  const int64_t row = blockIdx.x;  // (b, hq, s)
+  const int S = p.q_len, s = (int)(row % S), hq = (int)(row / S % p.num_q_heads), b = (int)(row / S / p.num_q_heads), lane = threadIdx.x;
+  const int len = walk_len(p, b), start = walk_start(p, b, len);
+  const int r = s * p.n_rep + hq % p.n_rep, r_first = r / rows_per_group * rows_per_group;
+  const Walk walk = walk_of(p, len, start, r_first / p.n_rep, (min(S * p.n_rep, r_first + rows_per_group) - 1) / p.n_rep);
+  const int n_parts = walk_parts(p, walk.total);
+  const float* ml = p.part_ml + row * p.max_parts * 2;
+  const float* po = p.part_o + row * p.max_parts * D;
+  float M = kNegInf;
+  for (int base = 0; base < n_parts; base += 64) M = fmaxf(M, base + lane < n_parts ? ml[2 * (base + lane)] : kNegInf);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) M = fmaxf(M, __shfl_xor(M, o, 64));
+  const float m_use = M == kNegInf ? 0.f : M;
+  float acc[PASSES][2], L = 0.f;
+#pragma unroll
+  for (int e = 0; e < PASSES; ++e) acc[e][0] = acc[e][1] = 0.f;
+  const int d0 = 2 * lane;
+  for (int base = 0; base < n_parts; base += 64) {
+    const bool mine = base + lane < n_parts;
+    const float w_mine = mine ? __builtin_amdgcn_exp2f(ml[2 * (base + lane)] - m_use) : 0.f, l_mine = mine ? ml[2 * (base + lane) + 1] : 0.f;
+    const int here = min(64, n_parts - base);
+    for (int j0 = 0; j0 < here; j0 += 8) {
+      u32x2 v[8][PASSES];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < PASSES; ++e) {
+          v[j][e] = u32x2{0u, 0u};
+          if (j0 + j < here && d0 + 128 * e < D) v[j][e] = *reinterpret_cast<const u32x2*>(po + (int64_t)(base + j0 + j) * D + d0 + 128 * e);
+        }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j0 + j < here) {
+          const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_mine), j0 + j));
+          L += w * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l_mine), j0 + j));
+#pragma unroll
+          for (int e = 0; e < PASSES; ++e) acc[e][0] += w * __uint_as_float(v[j][e][0]), acc[e][1] += w * __uint_as_float(v[j][e][1]);
+        }
+      }
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+  uint16_t* op = p.out + (int64_t)b * p.o_sb + (int64_t)hq * p.o_sh + (int64_t)s * p.o_ss + d0;
+#pragma unroll
+  for (int e = 0; e < PASSES; ++e)
+    if (d0 + 128 * e < D) *reinterpret_cast<uint32_t*>(op + 128 * e) = pack_bf16x2(acc[e][0] * inv, acc[e][1] * inv);
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------
+struct WalkShape {
+  int nqt, nw, n_qgroups, part_units, max_parts;
+  size_t bytes;  // of partial results
+};
+
+// workspace_bytes: what partial results may take (the context is cut over no more workgroups than fit).
+static WalkShape walk_shape(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, size_t workspace_bytes) {
+  WalkShape s;
+  const int64_t n_rep = a->num_q_heads / pool->num_kv_heads, tiles = (a->q_len * n_rep + 15) / 16;
+  s.nqt = tiles == 1 ? 1 : 2;
+  s.nw = pool->head_dim == 256 ? 2 : 4;
+  s.n_qgroups = (int)((tiles + s.nqt - 1) / s.nqt);
+  int64_t units = ((int64_t)a->max_seq_len + 31) / 32;
+  if (a->window > 0) units = std::min(units, ((int64_t)a->window + a->q_len) / 32 + 2 + a->sinks / 32 + 2);
+  units = std::max<int64_t>(units, 1);
+  const int64_t groups = (int64_t)a->batch * pool->num_kv_heads * s.n_qgroups, slots = (int64_t)compute_units() * 8 / s.nw;
+  // Enough workgroups to fill the GPU once, a unit per wave at least, and 4096 tokens at most, so that one long sequence
+  // among short ones is shared out.
+  int64_t per = a->partition_tokens > 0 ? a->partition_tokens / 32
+                                        : std::min<int64_t>(std::max<int64_t>(units * groups / slots, s.nw), 128);
+  per = (std::max<int64_t>(per, 1) + s.nw - 1) / s.nw * s.nw;
+  int64_t parts = (units + per - 1) / per;
+  const size_t one = (size_t)a->batch * a->num_q_heads * a->q_len * (pool->head_dim + 2) * sizeof(float);
+  if (parts > 1 && workspace_bytes / one < (size_t)parts) {
+    parts = std::max<int64_t>((int64_t)(workspace_bytes / one), 1);
+    per = (units + parts - 1) / parts;
+  }
+  s.part_units = (int)per, s.max_parts = (int)parts;
+  s.bytes = parts > 1 ? one * (size_t)parts : 0;
+  return s;
+}
+
+size_t walk_workspace_bytes(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a) {
+  return walk_shape(pool, a, ~(size_t)0).bytes;
+}
+
+template <int BITS, int D, int NQT>
+static void launch_walk_kernel(const WalkParams& p, bool masked, hipStream_t s) {
+  constexpr int NW = D == 256 ? 2 : 4, OCC = D == 256 ? 1 : 2;
+  const dim3 grid((unsigned)p.total_items), block(64 * NW);
+  if (masked) hipLaunchKernelGGL((walk_attn_kernel<BITS, D, NQT, true, NW, OCC>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((walk_attn_kernel<BITS, D, NQT, false, NW, OCC>), grid, block, 0, s, p);
+}
+
+int walk_kernel_name(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, char* out, size_t cap) {
+  const WalkShape sh = walk_shape(pool, a, a->workspace ? a->workspace_bytes : 0);
+  snprintf(out, cap, "pace_kv::walk_attn_kernel<%d, %d, %d, %s, %d, %d>", pool_is_q4(pool) ? 4 : 16, pool->head_dim, sh.nqt,
+           a->mask ? "true" : "false", sh.nw, pool->head_dim == 256 ? 1 : 2);
+  return PACE_KV_OK;
+}
+
+int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, const char* who, hipStream_t stream) {
+  if (a->workspace) PACE_REQUIRE(aligned16(a->workspace), "%s: workspace must be 16-byte aligned", who);
+  const WalkShape sh = walk_shape(pool, a, a->workspace ? a->workspace_bytes : 0);
+  WalkParams p = {};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_sb = a->q_stride_b, p.q_sh = a->q_stride_h, p.q_ss = a->q_stride_s;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.o_sb = a->o_stride_b, p.o_sh = a->o_stride_h, p.o_ss = a->o_stride_s;
+  p.kpool = static_cast<const uint16_t*>(pool->k), p.vpool = static_cast<const uint16_t*>(pool->v);
+  p.k_bs = pool->k_block_stride, p.k_hs = pool->k_head_stride, p.v_bs = pool->v_block_stride, p.v_hs = pool->v_head_stride;
+  p.num_blocks = pool->num_blocks, p.num_kv_heads = pool->num_kv_heads;
+  p.table = a->block_table, p.table_stride = a->table_stride;
+  p.seq_lens = a->seq_lens, p.len_bias = a->seq_len_bias, p.len_bias_dev = a->seq_len_bias_ptr, p.kv_start = a->kv_start;
+  p.mask = a->mask, p.mask_is_f32 = a->mask_dtype == PACE_DTYPE_F32, p.mask_len = a->mask_len;
+  p.m_sb = a->mask_stride_b, p.m_ss = a->mask_stride_s;
+  p.n_rep = a->num_q_heads / pool->num_kv_heads, p.q_len = a->q_len, p.num_q_heads = a->num_q_heads, p.batch = a->batch;
+  p.causal = a->causal;
+  p.scale = a->scale, p.scale_log2 = a->scale * kLog2e;
+  p.window = std::min(a->window, 1 << 30), p.sinks = std::min(a->sinks, 1 << 30);  // (sums with them stay below 2^31)
+  p.n_qgroups = sh.n_qgroups, p.part_units = sh.part_units, p.max_parts = sh.max_parts;
+  const size_t rows = (size_t)a->batch * a->num_q_heads * a->q_len;
+  PACE_REQUIRE(rows < ((size_t)1 << 31), "%s: too many query rows", who);
+  if (sh.max_parts > 1) {
+    p.part_o = static_cast<float*>(a->workspace);
+    p.part_ml = p.part_o + rows * sh.max_parts * pool->head_dim;
+  }
+  p.total_items = (long long)a->batch * sh.max_parts * pool->num_kv_heads * sh.n_qgroups;
+  PACE_REQUIRE(p.total_items < (1ll << 31), "%s: grid too large", who);
+  if (a->k_new)  // the new tokens first: they are read back from the pool like all others
+    if (int rc = pace_kv_append_paged_at(pool, a->k_new, a->v_new, a->new_stride_b, a->new_stride_h, a->new_stride_t, a->batch, a->n_new,
+                                         a->block_table, a->table_stride, a->seq_lens, a->seq_len_bias - a->n_new, a->seq_len_bias_ptr, stream))
+      return rc;
+  const bool masked = a->mask != nullptr, q4 = pool_is_q4(pool);
+  for_head_dim(pool->head_dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (q4) {
+      if (sh.nqt == 1) launch_walk_kernel<4, D, 1>(p, masked, stream); else launch_walk_kernel<4, D, 2>(p, masked, stream);
+    } else {
+      if (sh.nqt == 1) launch_walk_kernel<16, D, 1>(p, masked, stream); else launch_walk_kernel<16, D, 2>(p, masked, stream);
+    }
+    if (sh.max_parts > 1) hipLaunchKernelGGL(walk_merge_kernel<D>, dim3((unsigned)rows), dim3(64), 0, stream, p, 16 * sh.nqt);
+  });
+  PACE_HIP_CHECK(hipGetLastError());
+  return PACE_KV_OK;
+}
+
+}  // namespace pace_kv

@@ -14,8 +14,9 @@ _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "li
 
 BLOCK_TOKENS = 16
 DTYPE_F32, DTYPE_BF16 = 0, 1
-ABI_VERSION = 14
+ABI_VERSION = 15
 STATIC_SCRATCH_BYTES = 32 << 20  # PACE_PAGED_ATTN_STATIC_SCRATCH_BYTES
+ELEM_Q4 = 1  # PACE_KV_ELEM_Q4: pools of 4-bit rows, strides in bytes
 HEAD_DIMS = (64, 96, 128, 256)  # head sizes the pool kernels are built for
 
 EXPORTED_SYMBOLS = (
@@ -40,6 +41,7 @@ EXPORTED_SYMBOLS = (
     "pace_kv_plan_compaction_flags",
     "pace_paged_attn_workspace_bytes",
     "pace_paged_attn_workspace_bytes_for_parts",
+    "pace_paged_attn_workspace_for",
     "pace_paged_attn_decode",
     "pace_paged_attn_verify",
     "pace_paged_attn_verify_static",
@@ -64,7 +66,7 @@ class PoolDesc(Structure):
         ("num_kv_heads", c_int32),
         ("head_dim", c_int32),
         ("block_size", c_int32),
-        ("elem_bytes", c_int32),  # 0 / 2: bf16 slabs, 4: fp32 rows
+        ("elem_bytes", c_int32),  # 0 / 2: bf16 slabs, 4: fp32 rows, ELEM_Q4: 4-bit rows
         ("reserved", c_int32),
     ]
 
@@ -127,6 +129,8 @@ class PagedAttnArgs(Structure):
         ("seq_len_bias", c_int32),
         ("rope", POINTER(RopeDesc)),
         ("seq_len_bias_ptr", c_void_p),
+        ("window", c_int32),
+        ("sinks", c_int32),
     ]
 
 
@@ -224,6 +228,8 @@ def load() -> ctypes.CDLL:
     lib.pace_paged_attn_workspace_bytes_for_parts.restype = c_size_t
     lib.pace_paged_attn_workspace_bytes_for_parts.argtypes = [c_int32] * 5
     A = POINTER(PagedAttnArgs)
+    lib.pace_paged_attn_workspace_for.restype = c_size_t
+    lib.pace_paged_attn_workspace_for.argtypes = [P, A]
     lib.pace_paged_attn_decode.restype = ctypes.c_int
     lib.pace_paged_attn_decode.argtypes = [P, A, c_void_p]
     lib.pace_paged_attn_verify.restype = ctypes.c_int

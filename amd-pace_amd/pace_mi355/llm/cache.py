@@ -115,6 +115,14 @@ class PagedKVCache(KVCacheBase):
     ``shared`` lets the layers of a ``KVCacheManager`` use one block table.
     ``num_kv_heads`` (or ``n_rep``) tells the cache how a GQA-expanded input maps
     to stored heads; with neither, every input head is stored.
+
+    ``kv_bits=4`` keeps the rows in 4 bits with a step and a middle per 32 dims (bf16 models; the
+    format is described in ``include/pace_kv_hip.h``): a third of the memory and of the bytes a decode step reads.
+    Keys and values are quantised as they are appended, so a step attends to the quantised new token too.
+
+    ``window`` / ``sinks`` restrict what attention reads: the token at position ``p`` reads positions above
+    ``p - window`` and, besides, the first ``sinks`` tokens of its sequence (from ``kv_start`` on).  Both may be changed
+    between steps (``set_window``), per layer; what is stored does not depend on them.
     """
 
     def __init__(
@@ -125,7 +133,14 @@ class PagedKVCache(KVCacheBase):
         num_kv_heads: Optional[int] = None,
         n_rep: Optional[int] = None,
         num_blocks: Optional[int] = None,
+        kv_bits: int = 16,
+        window: Optional[int] = None,
+        sinks: int = 0,
     ):
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16 (rows in the model's own dtype); got {kv_bits}")
+        self.kv_bits = int(kv_bits)
+        self.set_window(window, sinks)
         self.max_seq_length = int(max_seq_length)
         self._shared = shared if shared is not None else {}
         self._cfg_kv_heads = num_kv_heads
@@ -166,6 +181,22 @@ class PagedKVCache(KVCacheBase):
     def lens(self, value: np.ndarray) -> None:
         self._lens = value
 
+    def set_window(self, window: Optional[int], sinks: int = 0) -> None:
+        """Let attention read the last ``window`` tokens and the first ``sinks`` ones only (``None``: all of them)."""
+        window = 0 if window is None else int(window)
+        if window < 0 or int(sinks) < 0 or (sinks and not window):
+            raise ValueError(f"window ({window}) must be positive or None, sinks ({sinks}) not negative and given with a window")
+        if window and getattr(self, "f32", False):
+            raise RuntimeError("a window over an fp32 pool is not supported")
+        if getattr(self, "pool", None) is not None:
+            self._flush()  # a held-back append or a captured step belongs to the window it was made for
+        self.window, self.sinks = window, int(sinks)
+
+    @property
+    def pool_desc(self) -> Optional[nat.PoolDesc]:
+        """The library's descriptor of this layer's pool (``None`` before the first update)."""
+        return self._desc
+
     # -- set-up -----------------------------------------------------------------
     def _lazy_init(self, key_states: torch.Tensor) -> None:
         if self.pool is not None:
@@ -178,6 +209,13 @@ class PagedKVCache(KVCacheBase):
         # read by the dense operator's fp32 kernel through the block table; the append rides in that launch when it
         # has up to 32 query rows per KV head (decode, short verify steps), the rotary embedding never does
         self.f32 = key_states.dtype == torch.float32
+        if self.f32 and self.kv_bits == 4:
+            self.f32 = False
+            raise RuntimeError("a 4-bit cache takes bf16 key/value states; got torch.float32")
+        if self.f32 and self.window:
+            self.f32 = False
+            raise RuntimeError("a window over an fp32 pool is not supported")
+        self.dtype = key_states.dtype
         nat.load()
         B, h_in, _, D = key_states.shape
         if self._cfg_kv_heads is not None:
@@ -203,7 +241,10 @@ class PagedKVCache(KVCacheBase):
         nb = self.state.allocator.num_blocks
         # [block][head][K|V][16*D]: one block of one layer is contiguous (64 KiB at 8 heads x 128 dims)
         # and the K and V slabs a wavefront reads together are adjacent.
-        self.pool = torch.zeros((nb, hkv, 2, BLOCK * D), dtype=key_states.dtype, device=key_states.device)
+        if self.kv_bits == 4:
+            self.pool = torch.zeros((nb, hkv, 2, 10 * D), dtype=torch.uint8, device=key_states.device)
+        else:
+            self.pool = torch.zeros((nb, hkv, 2, BLOCK * D), dtype=key_states.dtype, device=key_states.device)
         self.state.pools.append(self.pool)
         self._desc = self._describe(self.pool)
         self.state.pool_descs.append(self._desc)
@@ -220,9 +261,9 @@ class PagedKVCache(KVCacheBase):
             v_head_stride=pool.stride(1),
             num_blocks=nb,
             num_kv_heads=hkv,
-            head_dim=slab // BLOCK,
+            head_dim=slab // (10 if pool.dtype == torch.uint8 else BLOCK),
             block_size=BLOCK,
-            elem_bytes=pool.element_size(),
+            elem_bytes=pool.element_size(),  # (a byte: nat.ELEM_Q4)
         )
 
     # -- reference interface ----------------------------------------------------
@@ -280,13 +321,13 @@ class PagedKVCache(KVCacheBase):
             # (a rotary embedding then rotates the first rotary_dim <= model_dim dims of the padded rows, in a launch of
             # its own: inside the attention launch it needs rotary_dim == the pool's head size)
             k, v = (torch.nn.functional.pad(t, (0, self.head_dim - self.model_dim)) for t in (k, v))
-        if k.dtype != self.pool.dtype or v.dtype != self.pool.dtype:
-            raise RuntimeError(f"the cache holds {self.pool.dtype}; got {k.dtype} / {v.dtype}")
+        if k.dtype != self.dtype or v.dtype != self.dtype:
+            raise RuntimeError(f"the cache holds {self.dtype}; got {k.dtype} / {v.dtype}")
         ks = k.stride()
         per16 = 4 if self.f32 else 8  # elements in 16 bytes
         if ks[3] != 1 or ks != v.stride() or ks[0] % per16 or ks[1] % per16 or ks[2] % per16:
             k, v = k.contiguous(), v.contiguous()
-        if self.f32 and rope is not None:
+        if (self.f32 or self.kv_bits == 4 or self.window) and rope is not None:
             # rotated in a launch of its own; the attention call that follows does the same with its queries
             _, k = rope(None, k)
             self._query_rope, rope = rope, None
@@ -470,8 +511,8 @@ class PagedKVCache(KVCacheBase):
         L = int(self.lens.max(initial=0)) if pad_to is None else int(pad_to)
         shape = (self.batch, self.num_kv_heads * n_rep, L, self.head_dim)
         padded = self.head_dim != self.model_dim
-        k = torch.empty(shape, dtype=self.pool.dtype, device=self.pool.device)
-        v = torch.empty(shape, dtype=self.pool.dtype, device=self.pool.device)
+        k = torch.empty(shape, dtype=self.dtype, device=self.pool.device)
+        v = torch.empty(shape, dtype=self.dtype, device=self.pool.device)
         if L:
             st = self.state
             table, (lens_dev, bias) = st.device_table(), st.device_lens(self.lens)
@@ -513,8 +554,8 @@ class PagedKVCache(KVCacheBase):
         dev = self.pool.device
         cu_dev = torch.from_numpy(cu.astype(np.int32)).pin_memory().to(dev, non_blocking=True)
         shape = (total, self.num_kv_heads * n_rep, self.head_dim)
-        k = torch.empty(shape, dtype=self.pool.dtype, device=dev)
-        v = torch.empty(shape, dtype=self.pool.dtype, device=dev)
+        k = torch.empty(shape, dtype=self.dtype, device=dev)
+        v = torch.empty(shape, dtype=self.dtype, device=dev)
         if total:
             st = self.state
             table, (lens_dev, bias) = st.device_table(), st.device_lens(self.lens)
@@ -536,7 +577,7 @@ class PagedKVCache(KVCacheBase):
         (the causal mask ``pace/llm/models/llama.py:292-299`` builds); with an additive
         mask ``[B|1, 1, S|1, Lm]`` the mask alone decides, as in the reference.
         """
-        if query.dim() != 4 or not query.is_cuda or self.pool is None or query.dtype != self.pool.dtype:
+        if query.dim() != 4 or not query.is_cuda or self.pool is None or query.dtype != self.dtype:
             raise RuntimeError("paged attention expects a device tensor [B, Hq, S, D] of the cache's dtype (bf16 or fp32)")
         B, hq, S, D = query.shape
         if B != self.batch or D != self.model_dim or hq % self.num_kv_heads:
@@ -555,13 +596,15 @@ class PagedKVCache(KVCacheBase):
         if rope is not None:
             if tuple(rope.rows.shape) not in ((B, S), (1, S)):
                 raise RuntimeError(f"rope rows {tuple(rope.rows.shape)} do not match the query [B={B}, S={S}]")
-            rope_desc = None if self.f32 else rope.desc()
-            if self.f32:
+            own_launch = self.f32 or self.kv_bits == 4
+            rope_desc = None if own_launch else rope.desc()
+            if own_launch:
                 query, _ = rope(query, None)  # (the keys were rotated before their append)
                 qs = query.stride()
-            elif attention_mask is not None or rope_desc.rotary_dim != D:
+            elif attention_mask is not None or rope_desc.rotary_dim != D or self.window:
                 # cases the attention launch does not fold in: rotate the queries (and a held-back append) first
-                self._flush()
+                if self._pending is None or self._pending[3] is not None:
+                    self._flush()
                 query, _ = rope(query, None)
                 qs = query.stride()
                 rope_desc = None
@@ -579,7 +622,19 @@ class PagedKVCache(KVCacheBase):
         plan = lambda: st.plan_attention(self.lens, hq, self.num_kv_heads, self.head_dim, S, attention_mask is not None,
                                          self.partition_tokens)
         a = nat.PagedAttnArgs()
-        if self.f32:
+        walk = self.kv_bits == 4 or self.window > 0  # kernels that need no work list
+        if walk:
+            items = parts = None
+            n_items = max_parts = ws_bytes = 0  # (the library is asked for the workspace once the arguments are complete)
+            a.window, a.sinks = self.window, self.sinks
+            if graph is None:
+                table, (lens_dev, bias) = st.device_table(), st.device_lens(self.lens)
+                a.seq_len_bias = bias
+            else:  # captured step: as below
+                table, lens_dev = graph.table, graph.lens_dev
+                a.seq_len_bias, a.seq_len_bias_ptr = graph.new_tokens, graph.counter.data_ptr()
+                max_len = int(graph.base.max()) + graph.new_tokens * graph.max_steps
+        elif self.f32:
             # rows of fp32: one launch of the dense operator's kernel over the block table, no work list, no workspace
             items = parts = None
             n_items = max_parts = ws_bytes = 0
@@ -604,7 +659,6 @@ class PagedKVCache(KVCacheBase):
             table, lens_dev = graph.table, graph.lens_dev
             a.seq_len_bias, a.seq_len_bias_ptr = graph.new_tokens, graph.counter.data_ptr()
             max_len = int(graph.base.max()) + graph.new_tokens * graph.max_steps
-        ws = st.workspace(ws_bytes)
         a.q, a.q_stride_b, a.q_stride_h, a.q_stride_s = query.data_ptr(), qs[0], qs[1], qs[2]
         a.out, a.o_stride_b, a.o_stride_h, a.o_stride_s = out.data_ptr(), hq * S * D, S * D, D  # (allocated above: contiguous)
         a.block_table, a.table_stride = table.data_ptr(), table.stride(0)
@@ -627,11 +681,14 @@ class PagedKVCache(KVCacheBase):
         else:
             a.mask, a.causal = None, 1
         a.batch, a.num_q_heads, a.q_len = B, hq, S
-        a.max_seq_len, a.partition_tokens = max_len, 0
+        a.max_seq_len, a.partition_tokens = max_len, self.partition_tokens if walk else 0
         if items is not None:
             a.work_items, a.n_work_items = items.data_ptr(), n_items
             a.seq_parts, a.max_parts = parts.data_ptr(), max_parts
         a.scale = 1.0 / math.sqrt(self.model_dim)
+        if walk:
+            ws_bytes = int(lib.pace_paged_attn_workspace_for(ctypes.byref(self._desc), ctypes.byref(a)))
+        ws = st.workspace(ws_bytes)
         a.workspace = None if ws is None else ws.data_ptr()
         a.workspace_bytes = ws_bytes
         if rope_desc is not None:

@@ -41,6 +41,21 @@
  * workgroups); what folds other steps into
  * a launch (pace_rope_append_paged, args->rope, args->k_new) is bf16 only and
  * says so when handed such a pool.
+ *
+ * A pool may hold its rows in 4 bits (elem_bytes = PACE_KV_ELEM_Q4).  A row is
+ * cut into groups of 32 dims; a group holds a step s and a middle m (halves)
+ * and a code -8 .. 7 per value, and stands for s * code + m:
+ *   s = the least half with 15 s >= max - min,  m = half(min + 8 s),
+ *   code = round-half-even((x - m) / s) held in -8 .. 7 (0 where s = 0);
+ * NaN counts as 0 and values are held at +-32768 before that.  Slabs take
+ * 10 * head_dim bytes each for K and for V, head_dim as for bf16, strides in
+ * BYTES (multiples of 16).  New tokens, gathered rows, queries and outputs are
+ * bf16: append / append_paged / append_paged_at quantise, gather /
+ * gather_packed / gather_live read back, copy_blocks and compact_blocks move
+ * the slabs as they are, and the attention entry points read the codes in place
+ * (a fused append, args->k_new, is quantised first; no rotary embedding inside
+ * the launch; a work list is ignored).  In one append call no slot may be named
+ * twice.  Allocate the pool zero-filled.
  */
 #ifndef PACE_KV_HIP_H
 #define PACE_KV_HIP_H
@@ -60,6 +75,9 @@ enum {
   PACE_KV_EHIP = -2,   /* a HIP runtime call failed (launch, attribute query...) */
 };
 
+/* pace_kv_pool_t.elem_bytes of a pool of 4-bit rows */
+#define PACE_KV_ELEM_Q4 1
+
 enum { PACE_DTYPE_F32 = 0, PACE_DTYPE_BF16 = 1 };
 
 typedef struct pace_kv_pool {
@@ -73,7 +91,7 @@ typedef struct pace_kv_pool {
   int32_t num_kv_heads;
   int32_t head_dim;       /* bf16: 64, 96, 128 or 256; fp32: 4 .. 256, % 4   */
   int32_t block_size;     /* must be PACE_KV_BLOCK_TOKENS                    */
-  int32_t elem_bytes;     /* 0 or 2: bf16 slabs; 4: fp32 rows (see above)    */
+  int32_t elem_bytes;     /* 0 or 2: bf16 slabs; 4: fp32 rows; PACE_KV_ELEM_Q4: 4-bit rows, strides in bytes */
   int32_t reserved;       /* 0                                               */
 } pace_kv_pool_t;
 
@@ -349,6 +367,12 @@ typedef struct pace_paged_attn_args {
    * lengths between replays (a one-element increment kernel inside the graph).  max_seq_len must then
    * bound the lengths over all replays, and the block table must already hold their blocks. */
   const int32_t* seq_len_bias_ptr;
+  /* Optional window (0 = off; bf16 and 4-bit pools).  The query row at position pos = seq_len - q_len + s reads only
+   * tokens > pos - window, and besides them the first `sinks` tokens from kv_start on (sinks needs a window).  What the
+   * causal limit or the mask allows is not widened by it.  Only the tokens some row reads are fetched.  A windowed
+   * launch takes no rotary embedding and ignores a work list. */
+  int32_t window;
+  int32_t sinks;
 } pace_paged_attn_args_t;
 
 /* The context split size (tokens per workgroup) the library uses for these sizes when
@@ -409,6 +433,11 @@ int pace_paged_attn_kernel_name(const pace_kv_pool_t* pool, const pace_paged_att
 size_t pace_paged_attn_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t q_len,
                                        int32_t head_dim, int32_t max_seq_len,
                                        int32_t partition_tokens, int32_t num_kv_heads);
+
+/* The same for one particular call: the scratch pace_paged_attn_decode / _verify use for this pool and these arguments
+ * (whose workspace fields are not read).  Over a 4-bit pool or through a window less is accepted, and none at all:
+ * the context is then cut over fewer workgroups. */
+size_t pace_paged_attn_workspace_for(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* args);
 
 size_t pace_paged_attn_workspace_bytes_for_parts(int32_t batch, int32_t num_q_heads, int32_t q_len,
                                                  int32_t head_dim, int32_t max_parts);
