@@ -56,77 +56,160 @@ __device__ __forceinline__ int walk_len(const WalkParams& p, int b) {
 __device__ __forceinline__ int walk_start(const WalkParams& p, int b, int len) { return p.kv_start ? min(max(p.kv_start[b], 0), len) : 0; }
 __device__ __forceinline__ int walk_parts(const WalkParams& p, int total) { return min(max((total + p.part_units - 1) / p.part_units, 1), p.max_parts); }
 
-// ---- one unit of either pool ------------------------------------------------------------------------------------
+// ---- units of either pool ---------------------------------------------------------------------------------------
 template <int N>
 struct Dwords {
   typedef uint32_t type __attribute__((ext_vector_type(N), aligned(4)));
 };
 template <int N>
-__device__ __forceinline__ void load_dwords(uint32_t (&r)[N], const uint32_t* at) {
+__device__ __forceinline__ void load_dwords(uint32_t* r, const uint32_t* at) {
+  if constexpr (N == 1) {
+    r[0] = *at;
+  } else {
+    const typename Dwords<N>::type v = *reinterpret_cast<const typename Dwords<N>::type*>(at);
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = v[i];
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_dwords_once(uint32_t* r, const uint32_t* at) {  // nothing else will read them
   const typename Dwords<N>::type v = __builtin_nontemporal_load(reinterpret_cast<const typename Dwords<N>::type*>(at));
 #pragma unroll
   for (int i = 0; i < N; ++i) r[i] = v[i];
 }
-// (scales: sixteen lanes, or four, want the same bytes)
-template <int N>
-__device__ __forceinline__ void load_shared(uint32_t (&r)[N], const uint32_t* at) {
-  const typename Dwords<N>::type v = *reinterpret_cast<const typename Dwords<N>::type*>(at);
+
+// Eight K values of one token / eight V values of one dim from a code dword.
+__device__ __forceinline__ u32x4 q4_k_operand(uint32_t codes, uint32_t scale) {
+  const f16x2 sm = __builtin_bit_cast(f16x2, scale);
+  u32x4 r;
 #pragma unroll
-  for (int i = 0; i < N; ++i) r[i] = v[i];
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, q4_pair(codes, i, f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]}));
+  return r;
+}
+__device__ __forceinline__ u32x4 q4_v_operand(uint32_t codes, const uint32_t (&s)[4], const uint32_t (&m)[4]) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = __builtin_bit_cast(uint32_t, q4_pair(codes, i, __builtin_bit_cast(f16x2, s[i]), __builtin_bit_cast(f16x2, m[i])));
+  return r;
 }
 
+// Lane (n, g)'s slab of K / V in the unit of pool blocks idA, idB.
+__device__ __forceinline__ const uint32_t* q4_k_slab(const WalkParams& p, int kvh, int idA, int idB, int n) {
+  const int64_t a = (int64_t)idA * p.k_bs, b = (int64_t)idB * p.k_bs;  // wave-uniform products
+  return reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.kpool) + (n >= 8 ? b : a) + (int64_t)kvh * p.k_hs);
+}
+__device__ __forceinline__ const uint32_t* q4_v_slab(const WalkParams& p, int kvh, int idA, int idB, int g) {
+  const int64_t a = (int64_t)idA * p.v_bs, b = (int64_t)idB * p.v_bs;
+  return reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.vpool) + (g >= 2 ? b : a) + (int64_t)kvh * p.v_hs);
+}
+
+// A unit as one wave fetches it for itself.
 template <int BITS, int D>
 struct WalkUnit;
 
 template <int D>
 struct WalkUnit<16, D> {
   UnitRegs<D> r;
-  __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int n, int g) { load_unit<D, false>(r, p, kvh, idA, idB, n, g); }
+  __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int n, int g) { load_unit<D, true>(r, p, kvh, idA, idB, n, g); }
   __device__ __forceinline__ u32x4 k(int t, int kk) const { return r.k[t][kk]; }
   __device__ __forceinline__ u32x4 v(int j) const { return r.v[j]; }
+  __device__ __forceinline__ void drop(const u32x4& keep) {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) r.v[j] &= keep;
+  }
 };
 
 template <int D>
 struct WalkUnit<4, D> {
   using L = Q4<D>;
-  uint32_t kc[2][L::KN][L::KC];  // K codes: [tile][load][dword], step kk = load * KC + dword
-  uint32_t ks[2][L::KN][L::KC];  // K steps and middles of this lane's token
-  uint32_t vc[L::VN][L::VC];     // V codes: dim tile j = load * VC + dword
-  uint32_t vs[L::G][4], vm[L::G][4];  // V steps and middles of this lane's eight tokens, per group of dims
+  uint32_t kc[2][L::G], ks[2][L::G];  // codes and (step, middle) of this lane's token of either tile
+  uint32_t vc[2 * L::G];              // codes of this lane's dim of every dim tile
+  uint32_t vs[L::G][4], vm[L::G][4];  // steps and middles of this lane's eight tokens, per group of dims
   __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int n, int g) {
-    const int64_t ka = (int64_t)idA * p.k_bs, kb = (int64_t)idB * p.k_bs, va = (int64_t)idA * p.v_bs, vb = (int64_t)idB * p.v_bs;
-    const uint32_t* kp = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.kpool) + (n >= 8 ? kb : ka) + (int64_t)kvh * p.k_hs);
-    const uint32_t* vp = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.vpool) + (g >= 2 ? vb : va) + (int64_t)kvh * p.v_hs);
+    const uint32_t* kp = q4_k_slab(p, kvh, idA, idB, n);
+    const uint32_t* vp = q4_v_slab(p, kvh, idA, idB, g);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < L::KN; ++i) {
-        load_dwords<L::KC>(kc[t][i], kp + L::k_code(t, g, n & 7, i * L::KC));
-        load_shared<L::KC>(ks[t][i], kp + L::k_scale(t, n & 7, i * L::KC));
+      for (int i = 0; i < L::G; i += L::KC) {
+        load_dwords_once<L::KC>(kc[t] + i, kp + L::k_code(t, g, n & 7, i));
+        load_dwords<L::KC>(ks[t] + i, kp + L::k_scale(t, n & 7, i));
       }
 #pragma unroll
-    for (int i = 0; i < L::VN; ++i) load_dwords<L::VC>(vc[i], vp + L::v_code(g & 1, i * L::VC, n));
+    for (int j = 0; j < 2 * L::G; j += L::VC) load_dwords_once<L::VC>(vc + j, vp + L::v_code(g & 1, j, n));
 #pragma unroll
     for (int kk = 0; kk < L::G; ++kk) {
-      load_shared<4>(vs[kk], vp + L::v_scale(kk, 8 * (g & 1)) / 2);
-      load_shared<4>(vm[kk], vp + (L::v_scale(kk, 8 * (g & 1)) + 16 * L::G) / 2);
+      load_dwords<4>(vs[kk], vp + L::v_scale(kk, 8 * (g & 1)) / 2);
+      load_dwords<4>(vm[kk], vp + (L::v_scale(kk, 8 * (g & 1)) + 16 * L::G) / 2);
     }
   }
-  __device__ __forceinline__ u32x4 k(int t, int kk) const {
-    const f16x2 sm = __builtin_bit_cast(f16x2, ks[t][kk / L::KC][kk % L::KC]);
-    u32x4 r;
+  __device__ __forceinline__ u32x4 k(int t, int kk) const { return q4_k_operand(kc[t][kk], ks[t][kk]); }
+  __device__ __forceinline__ u32x4 v(int j) const { return q4_v_operand(vc[j], vs[j / 2], vm[j / 2]); }
+  __device__ __forceinline__ void drop(const u32x4&) {}  // (a 4-bit pool holds finite values only)
+};
+
+// A unit in LDS, shared by the waves of a workgroup: operands lane for lane.
+template <int D>
+struct StagedUnit {
+  const u32x4* at;  // this lane's 16 bytes of the first operand
+  __device__ __forceinline__ u32x4 k(int t, int kk) const { return at[(t * (D / 32) + kk) * 64]; }
+  __device__ __forceinline__ u32x4 v(int j) const { return at[(D / 16 + j) * 64]; }
+  __device__ __forceinline__ void drop(const u32x4&) {}
+};
+
+// A wave's quarter of a unit on its way into LDS: KPW of the K operands (tile wave & 1, steps kk0 ..) and VPW of the V operands
+// (dim tiles j0 ..).  Where the operands do not divide by four (head size 96) two waves make the same one.
+template <int BITS, int D>
+struct UnitShare {
+  using L = Q4<D>;
+  static constexpr int G = D / 32, PW = (G + 1) / 2, VG = (PW + 1) / 2;
+  uint32_t kc[BITS == 4 ? PW : 1], ks[BITS == 4 ? PW : 1], vc[BITS == 4 ? PW : 1], vs[BITS == 4 ? VG : 1][4], vm[BITS == 4 ? VG : 1][4];
+  u32x4 kr[BITS == 16 ? PW : 1], vr[BITS == 16 ? PW : 1];
+  __device__ static __forceinline__ int kk0(int wave) { return min((wave >> 1) * PW, G - PW); }
+  __device__ static __forceinline__ int j0(int wave) { return min(wave * PW, 2 * G - PW); }
+  __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int wave, int n, int g) {
+    const int t = wave & 1, kk = kk0(wave), j = j0(wave);
+    if constexpr (BITS == 16) {
+      const int64_t ka = (int64_t)idA * p.k_bs, kb = (int64_t)idB * p.k_bs, va = (int64_t)idA * p.v_bs, vb = (int64_t)idB * p.v_bs;
+      const uint16_t* kp = p.kpool + (n >= 8 ? kb : ka) + (int64_t)kvh * p.k_hs + g * 64 + (n & 7) * 8 + t * (D * 8);
+      const uint16_t* vp = p.vpool + (g >= 2 ? vb : va) + (int64_t)kvh * p.v_hs + ((g & 1) * 16 + n) * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = __builtin_bit_cast(uint32_t, q4_pair(kc[t][kk / L::KC][kk % L::KC], i, f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]}));
-    return r;
+      for (int i = 0; i < PW; ++i) {
+        kr[i] = *reinterpret_cast<const u32x4*>(kp + (kk + i) * 256);
+        vr[i] = *reinterpret_cast<const u32x4*>(vp + (j + i) * 256);
+      }
+    } else {
+      const uint32_t* kp = q4_k_slab(p, kvh, idA, idB, n);
+      const uint32_t* vp = q4_v_slab(p, kvh, idA, idB, g);
+      load_dwords<PW>(kc, kp + L::k_code(t, g, n & 7, kk));
+      load_dwords<PW>(ks, kp + L::k_scale(t, n & 7, kk));
+      if constexpr (L::VC % PW == 0) {
+        load_dwords<PW>(vc, vp + L::v_code(g & 1, j, n));
+      } else {
+#pragma unroll
+        for (int i = 0; i < PW; ++i) vc[i] = vp[L::v_code(g & 1, j + i, n)];
+      }
+#pragma unroll
+      for (int i = 0; i < VG; ++i) {
+        load_dwords<4>(vs[i], vp + L::v_scale(j / 2 + i, 8 * (g & 1)) / 2);
+        load_dwords<4>(vm[i], vp + (L::v_scale(j / 2 + i, 8 * (g & 1)) + 16 * G) / 2);
+      }
+    }
   }
-  __device__ __forceinline__ u32x4 v(int j) const {
-    u32x4 r;
+  // keep: see WalkUnit<16>::drop
+  __device__ __forceinline__ void put(u32x4* stage, int wave, int lane, const u32x4& keep) const {
+    const int t = wave & 1, kk = kk0(wave), j = j0(wave);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = __builtin_bit_cast(uint32_t, q4_pair(vc[j / L::VC][j % L::VC], i, __builtin_bit_cast(f16x2, vs[j / 2][i]),
-                                                  __builtin_bit_cast(f16x2, vm[j / 2][i])));
-    return r;
+    for (int i = 0; i < PW; ++i) {
+      if constexpr (BITS == 16) {
+        stage[(t * G + kk + i) * 64 + lane] = kr[i];
+        stage[(2 * G + j + i) * 64 + lane] = vr[i] & keep;
+      } else {
+        stage[(t * G + kk + i) * 64 + lane] = q4_k_operand(kc[i], ks[i]);
+        stage[(2 * G + j + i) * 64 + lane] = q4_v_operand(vc[i], vs[i / 2], vm[i / 2]);
+      }
+    }
   }
 };
 
@@ -148,6 +231,7 @@ struct WalkRows {
   float cn[NQT];   // score product -> natural units (with a mask tensor)
   int limit[NQT];  // last readable token (-1: no such row, or none)
   int low[NQT];    // with a window: first token of it
+  int s[NQT], hq[NQT];  // query token and head
   int64_t mask_off[NQT];
 };
 
@@ -185,13 +269,47 @@ __device__ __forceinline__ int walk_query(u32x4 (&q)[D / 32]) {
   }
 }
 
-// One unit: FULL = every row reads all of its 32 tokens.
-template <int BITS, int D, int NQT, bool HAS_MASK, bool FULL>
-__device__ __forceinline__ void walk_unit(const WalkUnit<BITS, D>& u, WalkRows<D, NQT>& st, int t0, int start, int sink_end, int row_low,
-                                          int row_end, int g, const MaskRegs<NQT>& mregs) {
+// Sets up tile qt's row: query operand, limits, empty softmax state.  Returns the row's last readable token (no row: none).
+template <int BITS, int D, int NQT, bool HAS_MASK>
+__device__ __forceinline__ int walk_row(const WalkParams& p, WalkRows<D, NQT>& st, int qt, int b, int kvh, int len, int r, int g) {
+  const int S = p.q_len;
+  const bool valid = r < S * p.n_rep;
+  const int s = valid ? r / p.n_rep : 0, hq = kvh * p.n_rep + (valid ? r % p.n_rep : 0), pos = len - S + s;
+  st.s[qt] = s, st.hq[qt] = hq;
+  st.limit[qt] = valid ? (p.causal ? pos : len - 1) : -1;
+  st.low[qt] = p.window > 0 ? pos - p.window + 1 : 0;
+  st.mask_off[qt] = HAS_MASK ? (int64_t)b * p.m_sb + (int64_t)s * p.m_ss : 0;
+  const uint16_t* qp = p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh + (int64_t)s * p.q_ss + 8 * g;
+#pragma unroll
+  for (int kk = 0; kk < D / 32; ++kk) st.q[qt][kk] = valid ? *reinterpret_cast<const u32x4*>(qp + kk * 32) : u32x4{0u, 0u, 0u, 0u};
+  const int up = walk_query<BITS, D>(st.q[qt]);
+  const float down = __uint_as_float((uint32_t)(127 - up) << 23);
+  st.cn[qt] = p.scale * down;
+  st.c[qt] = fminf(fmaxf(p.scale_log2 * down, 0x1p-126f), 0x1p126f);  // (not 0 or infinite: it multiplies -inf and 0)
+  st.m[qt] = kNegInf, st.m_top[qt] = kNegInf, st.m_neg[qt] = 0.f, st.l[qt] = 0.f;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) st.o[qt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  return valid ? st.limit[qt] : 0x7fffffff;
+}
+
+// Tokens of the unit at t0 that no row of a group reads (past its end, between the sinks and the window) may hold anything in a
+// 16-bit pool: their weight is 0, and 0 times infinity must not be added.  Mask of the lane's eight tokens' V values.
+__device__ __forceinline__ u32x4 walk_keep(int t0, int g, int start, int sink_end, int low, int end) {
+  u32x4 keep = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int t = t0 + 8 * g + e;
+    if (t < start || t >= end || (t < low && t >= sink_end)) keep[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+  }
+  return keep;
+}
+
+// One unit against the rows of a wave.  full (wave-uniform): every row reads all of its 32 tokens.
+template <int BITS, int D, int NQT, bool HAS_MASK, class Unit>
+__device__ __forceinline__ void walk_unit(const Unit& u, WalkRows<D, NQT>& st, bool full, int t0, int start, int sink_end, int g,
+                                          const MaskRegs<NQT>& mregs) {
 #pragma clang fp contract(off)
   constexpr int KK = D / 32, MT = D / 16;
-  const int base = t0 + 8 * g;  // this lane's first token
   f32x4 sc[NQT][2];
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt) sc[qt][0] = sc[qt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -203,28 +321,32 @@ __device__ __forceinline__ void walk_unit(const WalkUnit<BITS, D>& u, WalkRows<D
 #pragma unroll
       for (int qt = 0; qt < NQT; ++qt) sc[qt][t] = walk_mfma<BITS>(k, st.q[qt][kk], sc[qt][t]);
     }
+  if (HAS_MASK) {
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sc[qt][e >> 2][e & 3] = __builtin_fmaf(sc[qt][e >> 2][e & 3], st.cn[qt], mregs.a[qt][e]);
+  }
+  if (!full) {
+    const int base = t0 + 8 * g;  // this lane's first token
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) {
+      const int hi = st.limit[qt] - base, lo = start - base, wl = st.low[qt] - base, se = sink_end - base;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e > hi || e < lo || (e < wl && e >= se)) sc[qt][e >> 2][e & 3] = kNegInf;  // whatever the token holds
+    }
+  }
   u32x4 pb[NQT];
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt) {
     float s[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      s[e] = sc[qt][e >> 2][e & 3];
-      if (HAS_MASK) s[e] = __builtin_fmaf(s[e], st.cn[qt], mregs.a[qt][e]);
-    }
-    if (!FULL) {
-      const int hi = st.limit[qt] - base, lo = start - base, wl = st.low[qt] - base, se = sink_end - base;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e > hi || e < lo || (e < wl && e >= se)) s[e] = kNegInf;  // whatever the token holds
-    }
+    for (int e = 0; e < 8; ++e) s[e] = sc[qt][e >> 2][e & 3];
     const float c = HAS_MASK ? kLog2e : st.c[qt];
-    const float top = st.m_top[qt];
-    bool above = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) above = above || s[e] > top;
-    if (__any(above)) {  // the reference follows the maximum lazily, as in softmax_and_output
-      const float mx = row_max4(fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))));
+    const float mine = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    if (__any(mine > st.m_top[qt])) {  // the reference follows the maximum lazily, as in softmax_and_output
+      const float mx = row_max4(mine);
       const float m_old = st.m[qt], m_new = fmaxf(m_old, mx);
       const float m_use = m_new == kNegInf ? 0.f : m_new;
       const float alpha = __builtin_amdgcn_exp2f((m_old - m_use) * c);
@@ -248,45 +370,76 @@ __device__ __forceinline__ void walk_unit(const WalkUnit<BITS, D>& u, WalkRows<D
       else pb[qt][i] = pack_bf16x2(w[2 * i], w[2 * i + 1]);
     }
   }
-  // Tokens that no row of the wave reads (past the end, between the sinks and the window) may hold anything in a 16-bit pool: their
-  // weight is 0, and 0 times infinity must not be added.  A 4-bit pool holds finite values only.
-  u32x4 keep = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-  if (!FULL && BITS == 16) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int t = base + e;
-      if (t < start || t >= row_end || (t < row_low && t >= sink_end)) keep[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-    }
-  }
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
-    u32x4 v = u.v(j);
-    if (!FULL && BITS == 16) v &= keep;
+    const u32x4 v = u.v(j);
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) st.o[qt][j] = walk_mfma<BITS>(v, pb[qt], st.o[qt][j]);
   }
 }
 
+// Row sums over the four lanes of a row, running maximum in log2 units (-inf stays -inf).
+template <int D, int NQT, bool HAS_MASK>
+__device__ __forceinline__ void walk_finish(WalkRows<D, NQT>& st) {
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+    st.l[qt] += xor_lanes(st.l[qt], 16);
+    st.l[qt] += xor_lanes(st.l[qt], 32);
+    st.m[qt] *= HAS_MASK ? kLog2e : st.c[qt];
+  }
+}
+
+// A finished row: the output, or this partition's share of it.
+template <int D, int NQT>
+__device__ __forceinline__ void walk_store(const WalkParams& p, const WalkRows<D, NQT>& st, int qt, int b, int part, int g) {
+  const float l = st.l[qt];
+  if (p.max_parts == 1) {
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that read nothing is 0; NaN stays NaN
+    uint16_t* op = p.out + (int64_t)b * p.o_sb + (int64_t)st.hq[qt] * p.o_sh + (int64_t)st.s[qt] * p.o_ss + 4 * g;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      const f32x4 o = st.o[qt][j];
+      *reinterpret_cast<u32x2*>(op + 16 * j) = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+    }
+  } else {
+    const int64_t at = (((int64_t)b * p.num_q_heads + st.hq[qt]) * p.q_len + st.s[qt]) * p.max_parts + part;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * j + 4 * g) = st.o[qt][j];
+    if (g == 0) *reinterpret_cast<u32x2*>(p.part_ml + 2 * at) = u32x2{__float_as_uint(st.m[qt]), __float_as_uint(l)};
+  }
+}
+
+// Which (KV head, partition, row group, sequence) workgroup `item` is: KV head fastest, so that one head's K / V stay in one
+// XCD's L2; row groups from the last to the first, because under the causal limit the later rows read more and the longest
+// workgroups should not be the last to start.
+struct WalkItem {
+  int kvh, part, qg, b;
+};
+__device__ __forceinline__ WalkItem walk_item(const WalkParams& p) {
+  WalkItem w;
+  const uint32_t item = blockIdx.x, rest = item / (uint32_t)p.num_kv_heads;
+  w.kvh = (int)(item % (uint32_t)p.num_kv_heads);
+  w.part = (int)(rest % (uint32_t)p.max_parts);
+  const uint32_t bz = rest / (uint32_t)p.max_parts;
+  w.qg = p.n_qgroups - 1 - (int)(bz % (uint32_t)p.n_qgroups), w.b = (int)(bz / (uint32_t)p.n_qgroups);
+  return w;
+}
+
 // ---------------------------------------------------------------------------------
-// NW waves split a partition's units among themselves (wave w: units w, w + NW, ...) and merge through LDS.
+// Up to 16 query rows per KV head (decode): every wave walks units of its own.  NW waves split a partition's units (wave w:
+// units w, w + NW, ...), fetch one ahead, and merge through LDS.
 // ---------------------------------------------------------------------------------
-template <int BITS, int D, int NQT, bool HAS_MASK, int NW, int OCC>
+template <int BITS, int D, bool HAS_MASK, int NW, int OCC>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8))) void walk_attn_kernel(const WalkParams p) {
-  constexpr int KK = D / 32, MT = D / 16;
-  __shared__ float merge_buf[(NW / 2) * 16 * NQT * (D + 2)];
+  constexpr int MT = D / 16, ROW_F = D + 2, SLOT_F = 16 * ROW_F;
+  __shared__ float merge_buf[(NW / 2) * SLOT_F];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t item = blockIdx.x;  // KV head fastest (one head's K / V stay in one XCD's L2), then partition, row group, sequence
-  const int kvh = (int)(item % (uint32_t)p.num_kv_heads);
-  const uint32_t rest = item / (uint32_t)p.num_kv_heads;
-  const int part = (int)(rest % (uint32_t)p.max_parts);
-  const uint32_t bz = rest / (uint32_t)p.max_parts;
-  const int qg = (int)(bz % (uint32_t)p.n_qgroups), b = (int)(bz / (uint32_t)p.n_qgroups);
+  const WalkItem at = walk_item(p);
+  const int b = at.b, kvh = at.kvh, part = at.part;
   const int len = walk_len(p, b), start = walk_start(p, b, len);
   const int S = p.q_len, R = S * p.n_rep;
-  const int r_first = qg * NQT * 16, r_last = min(R, r_first + NQT * 16) - 1;
-  const int s_first = r_first / p.n_rep, s_last = r_last / p.n_rep;
-  const Walk walk = walk_of(p, len, start, s_first, s_last);
+  const Walk walk = walk_of(p, len, start, 0, S - 1);
   const int n_parts = walk_parts(p, walk.total);
   if (part >= n_parts) return;  // uniform over the workgroup
   const int i_begin = part * p.part_units, i_end = part == n_parts - 1 ? walk.total : min(i_begin + p.part_units, walk.total);
@@ -296,114 +449,150 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
   const int32_t* row = p.table + (int64_t)b * p.table_stride;
   auto fetch_ids = [&](int first) {
     const int i = i_begin + wave + NW * (first + (lane >> 1));
-    const int at = 2 * walk.unit(i) + (lane & 1);
-    const int id = i < i_end && at < p.table_stride ? row[at] : 0;
+    const int t = 2 * walk.unit(i) + (lane & 1);
+    const int id = i < i_end && t < p.table_stride ? row[t] : 0;
     return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
   };
-  int ids = fetch_ids(0);
+  int ids = n_mine > 0 ? fetch_ids(0) : 0;
+  WalkUnit<BITS, D> even, odd;
+  auto send = [&](WalkUnit<BITS, D>& u, int k) {
+    if (k != 0 && (k & 31) == 0) ids = fetch_ids(k);
+    u.load(p, kvh, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1), n, g);
+  };
+  if (n_mine > 0) send(even, 0);
 
-  WalkRows<D, NQT> st;
-  int row_s[NQT], row_h[NQT], min_limit = 0x7fffffff;
-#pragma unroll
-  for (int qt = 0; qt < NQT; ++qt) {
-    const int r = r_first + qt * 16 + n;
-    const bool valid = r < R;
-    const int s = valid ? r / p.n_rep : 0, hq = kvh * p.n_rep + (valid ? r % p.n_rep : 0), pos = len - S + s;
-    row_s[qt] = s, row_h[qt] = hq;
-    st.limit[qt] = valid ? (p.causal ? pos : len - 1) : -1;
-    st.low[qt] = p.window > 0 ? pos - p.window + 1 : 0;
-    if (valid) min_limit = min(min_limit, st.limit[qt]);
-    st.mask_off[qt] = HAS_MASK ? (int64_t)b * p.m_sb + (int64_t)s * p.m_ss : 0;
-    const uint16_t* qp = p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh + (int64_t)s * p.q_ss + 8 * g;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) st.q[qt][kk] = valid ? *reinterpret_cast<const u32x4*>(qp + kk * 32) : u32x4{0u, 0u, 0u, 0u};
-    const int up = walk_query<BITS, D>(st.q[qt]);
-    const float down = __uint_as_float((uint32_t)(127 - up) << 23);
-    st.cn[qt] = p.scale * down;
-    st.c[qt] = fminf(fmaxf(p.scale_log2 * down, 0x1p-126f), 0x1p126f);  // (not 0 or infinite: it multiplies -inf and 0)
-    st.m[qt] = kNegInf, st.m_top[qt] = kNegInf, st.m_neg[qt] = 0.f, st.l[qt] = 0.f;
-#pragma unroll
-    for (int j = 0; j < MT; ++j) st.o[qt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  WalkRows<D, 1> st;
+  int min_limit = walk_row<BITS, D, 1, HAS_MASK>(p, st, 0, b, kvh, len, n, g);
 #pragma unroll
   for (int o = 1; o < 16; o *= 2) min_limit = min(min_limit, __shfl_xor(min_limit, o, 64));
   min_limit = __builtin_amdgcn_readfirstlane(min_limit);
-  const int row_low = p.window > 0 ? len - S + s_first - p.window + 1 : 0;  // lowest window start of the group
-  const int max_low = p.window > 0 ? len - S + s_last - p.window + 1 : 0;   // highest
-  const int row_end = p.causal ? min(len, len - S + s_last + 1) : len;
+  const int row_low = p.window > 0 ? len - S - p.window + 1 : 0;  // the first row's window, and the last row's
+  const int max_low = p.window > 0 ? len - p.window : 0;
 
-  for (int k = 0; k < n_mine; ++k) {
-    if (k != 0 && (k & 31) == 0) ids = fetch_ids(k);
+  auto take = [&](WalkUnit<BITS, D>& u, int k) {
     const int t0 = 32 * walk.unit(i_begin + wave + NW * k);
-    MaskRegs<NQT> mregs;
-    if (HAS_MASK) load_mask_regs<NQT>(mregs, p, st.mask_off, t0, g);
-    WalkUnit<BITS, D> u;
-    u.load(p, kvh, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1), n, g);
+    MaskRegs<1> mregs;
+    if (HAS_MASK) load_mask_regs<1>(mregs, p, st.mask_off, t0, g);
     const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
-    if (full) walk_unit<BITS, D, NQT, HAS_MASK, true>(u, st, t0, start, walk.sink_end, row_low, row_end, g, mregs);
-    else walk_unit<BITS, D, NQT, HAS_MASK, false>(u, st, t0, start, walk.sink_end, row_low, row_end, g, mregs);
+    if (BITS == 16 && !full) u.drop(walk_keep(t0, g, start, walk.sink_end, row_low, len));
+    walk_unit<BITS, D, 1, HAS_MASK>(u, st, full, t0, start, walk.sink_end, g, mregs);
+  };
+  for (int k = 0; k < n_mine; k += 2) {
+    if (k + 1 < n_mine) send(odd, k + 1);
+    take(even, k);
+    if (k + 2 < n_mine) send(even, k + 2);
+    if (k + 1 < n_mine) take(odd, k + 1);
   }
-
-#pragma unroll
-  for (int qt = 0; qt < NQT; ++qt) {
-    st.l[qt] += xor_lanes(st.l[qt], 16);
-    st.l[qt] += xor_lanes(st.l[qt], 32);
-    st.m[qt] *= HAS_MASK ? kLog2e : st.c[qt];  // log2 units; -inf stays -inf
-  }
+  walk_finish<D, 1, HAS_MASK>(st);
   // Pairwise merge of the waves' states (fixed order: the same bits from call to call).
-  constexpr int ROW_F = D + 2, SLOT_F = 16 * NQT * ROW_F;
 #pragma unroll
   for (int stride = 1; stride < NW; stride *= 2) {
-    const int slot = wave / (2 * stride);
+    float* slot = merge_buf + wave / (2 * stride) * SLOT_F + n * ROW_F;
     const bool sender = (wave & (2 * stride - 1)) == stride, receiver = (wave & (2 * stride - 1)) == 0;
     if (sender) {
 #pragma unroll
-      for (int qt = 0; qt < NQT; ++qt) {
-        float* to = merge_buf + slot * SLOT_F + (qt * 16 + n) * ROW_F;
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) to[16 * j + 4 * g + i] = st.o[qt][j][i];
-        if (g == 0) to[D] = st.m[qt], to[D + 1] = st.l[qt];
-      }
+        for (int i = 0; i < 4; ++i) slot[16 * j + 4 * g + i] = st.o[0][j][i];
+      if (g == 0) slot[D] = st.m[0], slot[D + 1] = st.l[0];
     }
     __syncthreads();
     if (receiver) {
+      const float m_b = slot[D], l_b = slot[D + 1], m_new = fmaxf(st.m[0], m_b), m_use = m_new == kNegInf ? 0.f : m_new;
+      const float wa = __builtin_amdgcn_exp2f(st.m[0] - m_use), wb = __builtin_amdgcn_exp2f(m_b - m_use);
 #pragma unroll
-      for (int qt = 0; qt < NQT; ++qt) {
-        const float* from = merge_buf + slot * SLOT_F + (qt * 16 + n) * ROW_F;
-        const float m_b = from[D], l_b = from[D + 1], m_new = fmaxf(st.m[qt], m_b), m_use = m_new == kNegInf ? 0.f : m_new;
-        const float wa = __builtin_amdgcn_exp2f(st.m[qt] - m_use), wb = __builtin_amdgcn_exp2f(m_b - m_use);
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) st.o[qt][j][i] = st.o[qt][j][i] * wa + from[16 * j + 4 * g + i] * wb;
-        st.l[qt] = st.l[qt] * wa + l_b * wb;
-        st.m[qt] = m_new;
-      }
+        for (int i = 0; i < 4; ++i) st.o[0][j][i] = st.o[0][j][i] * wa + slot[16 * j + 4 * g + i] * wb;
+      st.l[0] = st.l[0] * wa + l_b * wb;
+      st.m[0] = m_new;
     }
     __syncthreads();
   }
-  if (wave != 0) return;
-#pragma unroll
-  for (int qt = 0; qt < NQT; ++qt) {
-    if (r_first + qt * 16 + n >= R) continue;
-    const float l = st.l[qt];
-    if (p.max_parts == 1) {
-      const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that read nothing is 0; NaN stays NaN
-      uint16_t* op = p.out + (int64_t)b * p.o_sb + (int64_t)row_h[qt] * p.o_sh + (int64_t)row_s[qt] * p.o_ss + 4 * g;
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const f32x4 o = st.o[qt][j];
-        *reinterpret_cast<u32x2*>(op + 16 * j) = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
-      }
-    } else {
-      const int64_t at = (((int64_t)b * p.num_q_heads + row_h[qt]) * S + row_s[qt]) * p.max_parts + part;
-#pragma unroll
-      for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * j + 4 * g) = st.o[qt][j];
-      if (g == 0) *reinterpret_cast<u32x2*>(p.part_ml + 2 * at) = u32x2{__float_as_uint(st.m[qt]), __float_as_uint(l)};
+  if (wave == 0 && n < R) walk_store(p, st, 0, b, part, g);
+}
+
+// ---------------------------------------------------------------------------------
+// More query rows (drafted tokens, chunks of a prompt): the four waves of a workgroup own NQT tiles of 16 rows each and walk the
+// units together.  Each wave fetches and unpacks a quarter of a unit and puts it into LDS in operand order, so that the
+// unpacking is paid once per workgroup; fetches run two units ahead of their use (one in registers, one in LDS), with
+// one barrier per unit.  A row's softmax state never leaves its wave.
+// ---------------------------------------------------------------------------------
+template <int BITS, int D, int NQT, bool HAS_MASK, int OCC>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) void walk_rows_kernel(const WalkParams p) {
+  constexpr int OPERANDS = D / 8;  // of a unit, 16 bytes per lane each
+  __shared__ __attribute__((aligned(16))) u32x4 stage[2][OPERANDS * 64];
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const WalkItem at = walk_item(p);
+  const int b = at.b, kvh = at.kvh, part = at.part;
+  const int len = walk_len(p, b), start = walk_start(p, b, len);
+  const int S = p.q_len, R = S * p.n_rep;
+  const int r_first = at.qg * NQT * 64, r_last = min(R, r_first + NQT * 64) - 1;  // the workgroup's rows
+  const int s_first = r_first / p.n_rep, s_last = r_last / p.n_rep;
+  const Walk walk = walk_of(p, len, start, s_first, s_last);
+  const int n_parts = walk_parts(p, walk.total);
+  if (part >= n_parts) return;  // uniform over the workgroup
+  const int i_begin = part * p.part_units, i_end = part == n_parts - 1 ? walk.total : min(i_begin + p.part_units, walk.total);
+  const int wg_low = p.window > 0 ? len - S + s_first - p.window + 1 : 0;  // what no row of the workgroup reads (see walk_keep)
+  const int wg_end = p.causal ? min(len, len - S + s_last + 1) : len;
+
+  const int32_t* row = p.table + (int64_t)b * p.table_stride;
+  auto fetch_ids = [&](int first) {  // pool blocks of units first .. first + 31, one per lane; never outside the pool
+    const int i = first + (lane >> 1);
+    const int t = 2 * walk.unit(i) + (lane & 1);
+    const int id = i < i_end && t < p.table_stride ? row[t] : 0;
+    return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
+  };
+  int ids = i_begin < i_end ? fetch_ids(i_begin) : 0, ids_first = i_begin;
+  UnitShare<BITS, D> share;
+  auto send = [&](int i) {
+    if (i - ids_first == 32) ids = fetch_ids(i), ids_first = i;
+    share.load(p, kvh, __builtin_amdgcn_readlane(ids, 2 * (i - ids_first)), __builtin_amdgcn_readlane(ids, 2 * (i - ids_first) + 1), wave, n, g);
+  };
+  auto put = [&](int i) {
+    u32x4 keep = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+    if (BITS == 16) {
+      const int t0 = 32 * walk.unit(i);
+      if (t0 < start || t0 + 32 > wg_end || t0 < wg_low) keep = walk_keep(t0, g, start, walk.sink_end, wg_low, wg_end);
     }
+    share.put(stage[(i - i_begin) & 1], wave, lane, keep);
+  };
+  if (i_begin < i_end) send(i_begin);
+
+  WalkRows<D, NQT> st;
+  const int w_first = r_first + wave * NQT * 16, w_last = min(R, w_first + NQT * 16) - 1;  // this wave's rows
+  const bool any_rows = w_first < R;
+  int min_limit = 0x7fffffff;
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) min_limit = min(min_limit, walk_row<BITS, D, NQT, HAS_MASK>(p, st, qt, b, kvh, len, w_first + qt * 16 + n, g));
+#pragma unroll
+  for (int o = 1; o < 16; o *= 2) min_limit = min(min_limit, __shfl_xor(min_limit, o, 64));
+  min_limit = __builtin_amdgcn_readfirstlane(min_limit);
+  const int row_low = p.window > 0 ? len - S + w_first / p.n_rep - p.window + 1 : 0;
+  const int max_low = p.window > 0 ? len - S + w_last / p.n_rep - p.window + 1 : 0;
+  const int row_end = !any_rows ? 0 : (p.causal ? min(len, len - S + w_last / p.n_rep + 1) : len);
+
+  if (i_begin < i_end) put(i_begin);
+  if (i_begin + 1 < i_end) send(i_begin + 1);
+  __syncthreads();
+  for (int i = i_begin; i < i_end; ++i) {
+    if (i + 1 < i_end) put(i + 1);  // (every wave has left that stage: the barrier of the turn before)
+    if (i + 2 < i_end) send(i + 2);
+    const int t0 = 32 * walk.unit(i);
+    if (t0 < row_end && (t0 + 32 > row_low || t0 < walk.sink_end)) {
+      MaskRegs<NQT> mregs;
+      if (HAS_MASK) load_mask_regs<NQT>(mregs, p, st.mask_off, t0, g);
+      const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
+      const StagedUnit<D> u = {&stage[(i - i_begin) & 1][lane]};
+      walk_unit<BITS, D, NQT, HAS_MASK>(u, st, full, t0, start, walk.sink_end, g, mregs);
+    }
+    __syncthreads();
   }
+  walk_finish<D, NQT, HAS_MASK>(st);
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt)
+    if (w_first + qt * 16 + n < R) walk_store(p, st, qt, b, part, g);
 }
 
 // out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partitions of a query row, one wave per row.  A lane fetches the
@@ -461,28 +650,36 @@ __global__ __launch_bounds__(64) void walk_merge_kernel(const WalkParams p, int3
 
 // ---- host -------------------------------------------------------------------------------------------------------
 struct WalkShape {
-  int nqt, nw, n_qgroups, part_units, max_parts;
-  size_t bytes;  // of partial results
+  int nqt;         // 0: walk_attn_kernel; else row tiles per wave of walk_rows_kernel
+  int group_rows;  // query rows per workgroup
+  int n_qgroups, part_units, max_parts;
+  size_t bytes;    // of partial results
 };
+
+constexpr int walk_waves(int head_dim) { return head_dim == 256 ? 2 : 4; }  // of a workgroup of walk_attn_kernel
+constexpr int walk_occ(int head_dim) { return head_dim == 256 ? 1 : 2; }
+constexpr int rows_occ(int head_dim, int nqt) { return head_dim == 256 || nqt > 1 ? 2 : 3; }
 
 // workspace_bytes: what partial results may take (the context is cut over no more workgroups than fit).
 static WalkShape walk_shape(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, size_t workspace_bytes) {
   WalkShape s;
-  const int64_t n_rep = a->num_q_heads / pool->num_kv_heads, tiles = (a->q_len * n_rep + 15) / 16;
-  s.nqt = tiles == 1 ? 1 : 2;
-  s.nw = pool->head_dim == 256 ? 2 : 4;
-  s.n_qgroups = (int)((tiles + s.nqt - 1) / s.nqt);
+  const int64_t rows = a->q_len * (int64_t)(a->num_q_heads / pool->num_kv_heads);
+  const int D = pool->head_dim;
+  s.nqt = rows <= 16 ? 0 : (rows <= 64 || D == 256 ? 1 : 2);
+  s.group_rows = s.nqt == 0 ? 16 : 64 * s.nqt;
+  s.n_qgroups = (int)((rows + s.group_rows - 1) / s.group_rows);
   int64_t units = ((int64_t)a->max_seq_len + 31) / 32;
   if (a->window > 0) units = std::min(units, ((int64_t)a->window + a->q_len) / 32 + 2 + a->sinks / 32 + 2);
   units = std::max<int64_t>(units, 1);
-  const int64_t groups = (int64_t)a->batch * pool->num_kv_heads * s.n_qgroups, slots = (int64_t)compute_units() * 8 / s.nw;
-  // Enough workgroups to fill the GPU once, a unit per wave at least, and 4096 tokens at most, so that one long sequence
+  const int64_t at_once = s.nqt == 0 ? walk_waves(D) : 1;  // units a workgroup works on side by side
+  const int64_t per_cu = s.nqt == 0 ? 4 * walk_occ(D) / walk_waves(D) : rows_occ(D, s.nqt);
+  const int64_t groups = (int64_t)a->batch * pool->num_kv_heads * s.n_qgroups, slots = compute_units() * per_cu;
+  // Enough workgroups to fill the GPU once, at least four units each, and 4096 tokens at most, so that one long sequence
   // among short ones is shared out.
-  int64_t per = a->partition_tokens > 0 ? a->partition_tokens / 32
-                                        : std::min<int64_t>(std::max<int64_t>(units * groups / slots, s.nw), 128);
-  per = (std::max<int64_t>(per, 1) + s.nw - 1) / s.nw * s.nw;
+  int64_t per = a->partition_tokens > 0 ? a->partition_tokens / 32 : std::min<int64_t>(std::max<int64_t>(units * groups / slots, 4), 128);
+  per = (std::max<int64_t>(per, 1) + at_once - 1) / at_once * at_once;
   int64_t parts = (units + per - 1) / per;
-  const size_t one = (size_t)a->batch * a->num_q_heads * a->q_len * (pool->head_dim + 2) * sizeof(float);
+  const size_t one = (size_t)a->batch * a->num_q_heads * a->q_len * (D + 2) * sizeof(float);
   if (parts > 1 && workspace_bytes / one < (size_t)parts) {
     parts = std::max<int64_t>((int64_t)(workspace_bytes / one), 1);
     per = (units + parts - 1) / parts;
@@ -496,18 +693,20 @@ size_t walk_workspace_bytes(const pace_kv_pool_t* pool, const pace_paged_attn_ar
   return walk_shape(pool, a, ~(size_t)0).bytes;
 }
 
-template <int BITS, int D, int NQT>
-static void launch_walk_kernel(const WalkParams& p, bool masked, hipStream_t s) {
-  constexpr int NW = D == 256 ? 2 : 4, OCC = D == 256 ? 1 : 2;
-  const dim3 grid((unsigned)p.total_items), block(64 * NW);
-  if (masked) hipLaunchKernelGGL((walk_attn_kernel<BITS, D, NQT, true, NW, OCC>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((walk_attn_kernel<BITS, D, NQT, false, NW, OCC>), grid, block, 0, s, p);
+template <int BITS, int D, bool HAS_MASK>
+static void launch_walk_kernel(const WalkParams& p, int nqt, hipStream_t s) {
+  const dim3 grid((unsigned)p.total_items);
+  if (nqt == 0) hipLaunchKernelGGL((walk_attn_kernel<BITS, D, HAS_MASK, walk_waves(D), walk_occ(D)>), grid, dim3(64 * walk_waves(D)), 0, s, p);
+  else if (nqt == 1) hipLaunchKernelGGL((walk_rows_kernel<BITS, D, 1, HAS_MASK, rows_occ(D, 1)>), grid, dim3(256), 0, s, p);
+  else if constexpr (D != 256) hipLaunchKernelGGL((walk_rows_kernel<BITS, D, 2, HAS_MASK, rows_occ(D, 2)>), grid, dim3(256), 0, s, p);
 }
 
 int walk_kernel_name(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, char* out, size_t cap) {
   const WalkShape sh = walk_shape(pool, a, a->workspace ? a->workspace_bytes : 0);
-  snprintf(out, cap, "pace_kv::walk_attn_kernel<%d, %d, %d, %s, %d, %d>", pool_is_q4(pool) ? 4 : 16, pool->head_dim, sh.nqt,
-           a->mask ? "true" : "false", sh.nw, pool->head_dim == 256 ? 1 : 2);
+  const int bits = pool_is_q4(pool) ? 4 : 16, D = pool->head_dim;
+  const char* masked = a->mask ? "true" : "false";
+  if (sh.nqt == 0) snprintf(out, cap, "pace_kv::walk_attn_kernel<%d, %d, %s, %d, %d>", bits, D, masked, walk_waves(D), walk_occ(D));
+  else snprintf(out, cap, "pace_kv::walk_rows_kernel<%d, %d, %d, %s, %d>", bits, D, sh.nqt, masked, rows_occ(D, sh.nqt));
   return PACE_KV_OK;
 }
 
@@ -547,11 +746,11 @@ int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, con
   for_head_dim(pool->head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (q4) {
-      if (sh.nqt == 1) launch_walk_kernel<4, D, 1>(p, masked, stream); else launch_walk_kernel<4, D, 2>(p, masked, stream);
+      if (masked) launch_walk_kernel<4, D, true>(p, sh.nqt, stream); else launch_walk_kernel<4, D, false>(p, sh.nqt, stream);
     } else {
-      if (sh.nqt == 1) launch_walk_kernel<16, D, 1>(p, masked, stream); else launch_walk_kernel<16, D, 2>(p, masked, stream);
+      if (masked) launch_walk_kernel<16, D, true>(p, sh.nqt, stream); else launch_walk_kernel<16, D, false>(p, sh.nqt, stream);
     }
-    if (sh.max_parts > 1) hipLaunchKernelGGL(walk_merge_kernel<D>, dim3((unsigned)rows), dim3(64), 0, stream, p, 16 * sh.nqt);
+    if (sh.max_parts > 1) hipLaunchKernelGGL(walk_merge_kernel<D>, dim3((unsigned)rows), dim3(64), 0, stream, p, sh.group_rows);
   });
   PACE_HIP_CHECK(hipGetLastError());
   return PACE_KV_OK;
