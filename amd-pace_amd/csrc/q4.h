@@ -17,7 +17,7 @@
 //   V codes   [token half 2][dim tile quad][dim 16][dim tile] dwords: eight tokens of one dim
 //   V scales  [kk][token 16] halves: s, then the same of m
 // Value e of a dword sits at bit 4 (e / 2) + 16 (e & 1): a shift by 4 i brings values 2 i and 2 i + 1 to the low bits of the
-// two 16-bit halves, where `and 0x000f000f, or 0x64006400` makes them the halves 1024 + (code + 8).
+// two 16-bit halves (see q4_codes).
 #pragma once
 #include "common.h"
 
@@ -62,12 +62,24 @@ __device__ __forceinline__ _Float16 half_from(uint32_t b) { return __builtin_bit
 // Value e of a code dword as the number it is, -8 .. 7.
 __device__ __forceinline__ float q4_code(uint32_t w, int e) { return (float)((int)((w >> q4_bit(e)) & 15u) - 8); }
 
-// Eight codes -> the eight values they stand for, as halves in element order: s and m are the step and the middle of each
-// value pair's two values (both halves equal where the eight values share them).  One rounding, to half: code - 8 is
-// exact (a whole number up to 1039 in a half), and the multiply-add is fused.
-__device__ __forceinline__ f16x2 q4_pair(uint32_t w, int i, f16x2 s, f16x2 m) {
-  const f16x2 c = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) + f16x2{(_Float16)-1032.f, (_Float16)-1032.f};
-  return __builtin_elementwise_fma(c, s, m);
+// The eight codes of a dword as halves -8 .. 7, in element order.  `and-or` with the bits of 1024 makes a pair of halves 1024 +
+// (code + 8) of the low nibbles and 1024 + 16 (code + 8) of the next ones; one packed add or multiply-add takes the
+// offset out again, exactly.  One shift per dword and 2 instructions per pair; `or_bits` comes from q4_or_bits().
+__device__ __forceinline__ void q4_codes(uint32_t w, uint32_t or_bits, f16x2 (&c)[4]) {
+  const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = w >> (8 * i);
+    c[2 * i] = __builtin_bit_cast(f16x2, (x & 0x000f000fu) | or_bits) + f16x2{(_Float16)-1032.f, (_Float16)-1032.f};
+    c[2 * i + 1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (x & 0x00f000f0u) | or_bits), sixteenth, f16x2{(_Float16)-72.f, (_Float16)-72.f});
+  }
+}
+// 0x64006400 in a vector register: an instruction takes one constant from outside them, so that with both the mask and this one
+// outside, `and-or` would be two.
+__device__ __forceinline__ uint32_t q4_or_bits() {
+  uint32_t b = 0x64006400u;
+  asm volatile("" : "+v"(b));
+  return b;
 }
 
 // Quantises a group of 32 values held by four neighbouring lanes (eight each, lanes 4 k .. 4 k + 3): this lane's codes as

@@ -78,30 +78,45 @@ __device__ __forceinline__ void load_dwords_once(uint32_t* r, const uint32_t* at
   for (int i = 0; i < N; ++i) r[i] = v[i];
 }
 
-// Eight K values of one token / eight V values of one dim from a code dword.
-__device__ __forceinline__ u32x4 q4_k_operand(uint32_t codes, uint32_t scale) {
+// Eight K values of one token / eight V values of one dim from a code dword: one multiply-add per pair, rounded once, to half.
+__device__ __forceinline__ u32x4 q4_k_operand(uint32_t codes, uint32_t scale, uint32_t or_bits) {
   const f16x2 sm = __builtin_bit_cast(f16x2, scale);
+  f16x2 c[4];
+  q4_codes(codes, or_bits, c);
   u32x4 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, q4_pair(codes, i, f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]}));
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[i], f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]}));
   return r;
 }
-__device__ __forceinline__ u32x4 q4_v_operand(uint32_t codes, const uint32_t (&s)[4], const uint32_t (&m)[4]) {
+__device__ __forceinline__ u32x4 q4_v_operand(uint32_t codes, const uint32_t (&s)[4], const uint32_t (&m)[4], uint32_t or_bits) {
+  f16x2 c[4];
+  q4_codes(codes, or_bits, c);
   u32x4 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    r[i] = __builtin_bit_cast(uint32_t, q4_pair(codes, i, __builtin_bit_cast(f16x2, s[i]), __builtin_bit_cast(f16x2, m[i])));
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[i], __builtin_bit_cast(f16x2, s[i]), __builtin_bit_cast(f16x2, m[i])));
   return r;
 }
 
-// Lane (n, g)'s slab of K / V in the unit of pool blocks idA, idB.
-__device__ __forceinline__ const uint32_t* q4_k_slab(const WalkParams& p, int kvh, int idA, int idB, int n) {
-  const int64_t a = (int64_t)idA * p.k_bs, b = (int64_t)idB * p.k_bs;  // wave-uniform products
-  return reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.kpool) + (n >= 8 ? b : a) + (int64_t)kvh * p.k_hs);
+// Byte offsets of a unit's two blocks in K and in V.  They are products of wave-uniform numbers; left to itself the compiler
+// multiplies after the lanes have picked their block, in vector registers at a quarter of the rate.
+struct UnitOffsets {
+  int64_t ka, kb, va, vb;
+};
+template <int BITS>
+__device__ __forceinline__ UnitOffsets unit_offsets(const WalkParams& p, int idA, int idB) {
+  constexpr int64_t SIZE = BITS == 4 ? 1 : 2;
+  UnitOffsets u = {idA * p.k_bs * SIZE, idB * p.k_bs * SIZE, idA * p.v_bs * SIZE, idB * p.v_bs * SIZE};
+  asm volatile("" : "+s"(u.ka), "+s"(u.kb), "+s"(u.va), "+s"(u.vb));
+  return u;
 }
-__device__ __forceinline__ const uint32_t* q4_v_slab(const WalkParams& p, int kvh, int idA, int idB, int g) {
-  const int64_t a = (int64_t)idA * p.v_bs, b = (int64_t)idB * p.v_bs;
-  return reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.vpool) + (g >= 2 ? b : a) + (int64_t)kvh * p.v_hs);
+// Lane addresses that do not depend on the unit.
+struct LaneBase {
+  const char *kc, *ks, *vc, *vs;  // 4-bit pools: codes and scales of K and of V; 16-bit pools: kc and vc
+};
+template <class T>
+__device__ __forceinline__ const T* unit_at(const char* base, int64_t off) {
+  return reinterpret_cast<const T*>(base + off);
 }
 
 // A unit as one wave fetches it for itself.
@@ -111,7 +126,21 @@ struct WalkUnit;
 template <int D>
 struct WalkUnit<16, D> {
   UnitRegs<D> r;
-  __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int n, int g) { load_unit<D, true>(r, p, kvh, idA, idB, n, g); }
+  // (the operand layout of load_unit; nothing else reads these bytes in this launch)
+  __device__ static __forceinline__ LaneBase base(const WalkParams& p, int kvh, int n, int g) {
+    return {reinterpret_cast<const char*>(p.kpool + (int64_t)kvh * p.k_hs + g * 64 + (n & 7) * 8), nullptr,
+            reinterpret_cast<const char*>(p.vpool + (int64_t)kvh * p.v_hs + ((g & 1) * 16 + n) * 8), nullptr};
+  }
+  __device__ __forceinline__ void load(const LaneBase& lb, const UnitOffsets& o, int n, int g) {
+    const uint16_t* kp = unit_at<uint16_t>(lb.kc, n >= 8 ? o.kb : o.ka);
+    const uint16_t* vp = unit_at<uint16_t>(lb.vc, g >= 2 ? o.vb : o.va);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int kk = 0; kk < D / 32; ++kk) r.k[t][kk] = load16_stream(kp + t * (D * 8) + kk * 256);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) r.v[j] = load16_stream(vp + j * 256);
+  }
   __device__ __forceinline__ u32x4 k(int t, int kk) const { return r.k[t][kk]; }
   __device__ __forceinline__ u32x4 v(int j) const { return r.v[j]; }
   __device__ __forceinline__ void drop(const u32x4& keep) {
@@ -126,26 +155,33 @@ struct WalkUnit<4, D> {
   uint32_t kc[2][L::G], ks[2][L::G];  // codes and (step, middle) of this lane's token of either tile
   uint32_t vc[2 * L::G];              // codes of this lane's dim of every dim tile
   uint32_t vs[L::G][4], vm[L::G][4];  // steps and middles of this lane's eight tokens, per group of dims
-  __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int n, int g) {
-    const uint32_t* kp = q4_k_slab(p, kvh, idA, idB, n);
-    const uint32_t* vp = q4_v_slab(p, kvh, idA, idB, g);
+  uint32_t or_bits;
+  __device__ static __forceinline__ LaneBase base(const WalkParams& p, int kvh, int n, int g) {
+    const char* k = reinterpret_cast<const char*>(p.kpool) + (int64_t)kvh * p.k_hs;
+    const char* v = reinterpret_cast<const char*>(p.vpool) + (int64_t)kvh * p.v_hs;
+    return {k + 4 * L::k_code(0, g, n & 7, 0), k + 4 * L::k_scale(0, n & 7, 0), v + 4 * L::v_code(g & 1, 0, n), v + 2 * L::v_scale(0, 8 * (g & 1))};
+  }
+  __device__ __forceinline__ void load(const LaneBase& lb, const UnitOffsets& o, int n, int g) {
+    const int64_t ko = n >= 8 ? o.kb : o.ka, vo = g >= 2 ? o.vb : o.va;
+    const uint32_t *kc_at = unit_at<uint32_t>(lb.kc, ko), *ks_at = unit_at<uint32_t>(lb.ks, ko);
+    const uint32_t *vc_at = unit_at<uint32_t>(lb.vc, vo), *vs_at = unit_at<uint32_t>(lb.vs, vo);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < L::G; i += L::KC) {
-        load_dwords_once<L::KC>(kc[t] + i, kp + L::k_code(t, g, n & 7, i));
-        load_dwords<L::KC>(ks[t] + i, kp + L::k_scale(t, n & 7, i));
+        load_dwords_once<L::KC>(kc[t] + i, kc_at + (L::k_code(t, 0, 0, i) - L::k_code(0, 0, 0, 0)));
+        load_dwords<L::KC>(ks[t] + i, ks_at + (L::k_scale(t, 0, i) - L::k_scale(0, 0, 0)));
       }
 #pragma unroll
-    for (int j = 0; j < 2 * L::G; j += L::VC) load_dwords_once<L::VC>(vc + j, vp + L::v_code(g & 1, j, n));
+    for (int j = 0; j < 2 * L::G; j += L::VC) load_dwords_once<L::VC>(vc + j, vc_at + (L::v_code(0, j, 0) - L::v_code(0, 0, 0)));
 #pragma unroll
     for (int kk = 0; kk < L::G; ++kk) {
-      load_dwords<4>(vs[kk], vp + L::v_scale(kk, 8 * (g & 1)) / 2);
-      load_dwords<4>(vm[kk], vp + (L::v_scale(kk, 8 * (g & 1)) + 16 * L::G) / 2);
+      load_dwords<4>(vs[kk], vs_at + 8 * kk);
+      load_dwords<4>(vm[kk], vs_at + 8 * (kk + L::G));
     }
   }
-  __device__ __forceinline__ u32x4 k(int t, int kk) const { return q4_k_operand(kc[t][kk], ks[t][kk]); }
-  __device__ __forceinline__ u32x4 v(int j) const { return q4_v_operand(vc[j], vs[j / 2], vm[j / 2]); }
+  __device__ __forceinline__ u32x4 k(int t, int kk) const { return q4_k_operand(kc[t][kk], ks[t][kk], or_bits); }
+  __device__ __forceinline__ u32x4 v(int j) const { return q4_v_operand(vc[j], vs[j / 2], vm[j / 2], or_bits); }
   __device__ __forceinline__ void drop(const u32x4&) {}  // (a 4-bit pool holds finite values only)
 };
 
@@ -168,37 +204,47 @@ struct UnitShare {
   u32x4 kr[BITS == 16 ? PW : 1], vr[BITS == 16 ? PW : 1];
   __device__ static __forceinline__ int kk0(int wave) { return min((wave >> 1) * PW, G - PW); }
   __device__ static __forceinline__ int j0(int wave) { return min(wave * PW, 2 * G - PW); }
-  __device__ __forceinline__ void load(const WalkParams& p, int kvh, int idA, int idB, int wave, int n, int g) {
+  __device__ static __forceinline__ LaneBase base(const WalkParams& p, int kvh, int wave, int n, int g) {
     const int t = wave & 1, kk = kk0(wave), j = j0(wave);
     if constexpr (BITS == 16) {
-      const int64_t ka = (int64_t)idA * p.k_bs, kb = (int64_t)idB * p.k_bs, va = (int64_t)idA * p.v_bs, vb = (int64_t)idB * p.v_bs;
-      const uint16_t* kp = p.kpool + (n >= 8 ? kb : ka) + (int64_t)kvh * p.k_hs + g * 64 + (n & 7) * 8 + t * (D * 8);
-      const uint16_t* vp = p.vpool + (g >= 2 ? vb : va) + (int64_t)kvh * p.v_hs + ((g & 1) * 16 + n) * 8;
+      return {reinterpret_cast<const char*>(p.kpool + (int64_t)kvh * p.k_hs + g * 64 + (n & 7) * 8 + t * (D * 8) + kk * 256), nullptr,
+              reinterpret_cast<const char*>(p.vpool + (int64_t)kvh * p.v_hs + ((g & 1) * 16 + n) * 8 + j * 256), nullptr};
+    } else {
+      const char* k = reinterpret_cast<const char*>(p.kpool) + (int64_t)kvh * p.k_hs;
+      const char* v = reinterpret_cast<const char*>(p.vpool) + (int64_t)kvh * p.v_hs;
+      return {k + 4 * L::k_code(t, g, n & 7, kk), k + 4 * L::k_scale(t, n & 7, kk), v + 4 * L::v_code(g & 1, j, n), v + 2 * L::v_scale(j / 2, 8 * (g & 1))};
+    }
+  }
+  __device__ __forceinline__ void load(const LaneBase& lb, const UnitOffsets& o, int wave, int n, int g) {
+    const int64_t ko = n >= 8 ? o.kb : o.ka, vo = g >= 2 ? o.vb : o.va;
+    if constexpr (BITS == 16) {
+      const uint16_t *kp = unit_at<uint16_t>(lb.kc, ko), *vp = unit_at<uint16_t>(lb.vc, vo);
 #pragma unroll
       for (int i = 0; i < PW; ++i) {
-        kr[i] = *reinterpret_cast<const u32x4*>(kp + (kk + i) * 256);
-        vr[i] = *reinterpret_cast<const u32x4*>(vp + (j + i) * 256);
+        kr[i] = *reinterpret_cast<const u32x4*>(kp + i * 256);
+        vr[i] = *reinterpret_cast<const u32x4*>(vp + i * 256);
       }
     } else {
-      const uint32_t* kp = q4_k_slab(p, kvh, idA, idB, n);
-      const uint32_t* vp = q4_v_slab(p, kvh, idA, idB, g);
-      load_dwords<PW>(kc, kp + L::k_code(t, g, n & 7, kk));
-      load_dwords<PW>(ks, kp + L::k_scale(t, n & 7, kk));
+      load_dwords<PW>(kc, unit_at<uint32_t>(lb.kc, ko));
+      load_dwords<PW>(ks, unit_at<uint32_t>(lb.ks, ko));
+      const uint32_t* vc_at = unit_at<uint32_t>(lb.vc, vo);
       if constexpr (L::VC % PW == 0) {
-        load_dwords<PW>(vc, vp + L::v_code(g & 1, j, n));
+        load_dwords<PW>(vc, vc_at);
       } else {
+        const int j = j0(wave);
 #pragma unroll
-        for (int i = 0; i < PW; ++i) vc[i] = vp[L::v_code(g & 1, j + i, n)];
+        for (int i = 0; i < PW; ++i) vc[i] = vc_at[L::v_code(0, j + i, 0) - L::v_code(0, j, 0)];
       }
+      const uint32_t* vs_at = unit_at<uint32_t>(lb.vs, vo);
 #pragma unroll
       for (int i = 0; i < VG; ++i) {
-        load_dwords<4>(vs[i], vp + L::v_scale(j / 2 + i, 8 * (g & 1)) / 2);
-        load_dwords<4>(vm[i], vp + (L::v_scale(j / 2 + i, 8 * (g & 1)) + 16 * G) / 2);
+        load_dwords<4>(vs[i], vs_at + 8 * i);
+        load_dwords<4>(vm[i], vs_at + 8 * (i + G));
       }
     }
   }
   // keep: see WalkUnit<16>::drop
-  __device__ __forceinline__ void put(u32x4* stage, int wave, int lane, const u32x4& keep) const {
+  __device__ __forceinline__ void put(u32x4* stage, int wave, int lane, const u32x4& keep, uint32_t or_bits) const {
     const int t = wave & 1, kk = kk0(wave), j = j0(wave);
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
@@ -206,8 +252,8 @@ struct UnitShare {
         stage[(t * G + kk + i) * 64 + lane] = kr[i];
         stage[(2 * G + j + i) * 64 + lane] = vr[i] & keep;
       } else {
-        stage[(t * G + kk + i) * 64 + lane] = q4_k_operand(kc[i], ks[i]);
-        stage[(2 * G + j + i) * 64 + lane] = q4_v_operand(vc[i], vs[i / 2], vm[i / 2]);
+        stage[(t * G + kk + i) * 64 + lane] = q4_k_operand(kc[i], ks[i], or_bits);
+        stage[(2 * G + j + i) * 64 + lane] = q4_v_operand(vc[i], vs[i / 2], vm[i / 2], or_bits);
       }
     }
   }
@@ -299,7 +345,7 @@ __device__ __forceinline__ u32x4 walk_keep(int t0, int g, int start, int sink_en
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int t = t0 + 8 * g + e;
-    if (t < start || t >= end || (t < low && t >= sink_end)) keep[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+    if ((t < start) | (t >= end) | ((t < low) & (t >= sink_end))) keep[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
   }
   return keep;
 }
@@ -334,7 +380,7 @@ __device__ __forceinline__ void walk_unit(const Unit& u, WalkRows<D, NQT>& st, b
       const int hi = st.limit[qt] - base, lo = start - base, wl = st.low[qt] - base, se = sink_end - base;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (e > hi || e < lo || (e < wl && e >= se)) sc[qt][e >> 2][e & 3] = kNegInf;  // whatever the token holds
+        sc[qt][e >> 2][e & 3] = (e > hi) | (e < lo) | ((e < wl) & (e >= se)) ? kNegInf : sc[qt][e >> 2][e & 3];  // whatever the token holds
     }
   }
   u32x4 pb[NQT];
@@ -454,10 +500,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
   };
   int ids = n_mine > 0 ? fetch_ids(0) : 0;
+  const LaneBase base = WalkUnit<BITS, D>::base(p, kvh, n, g);
   WalkUnit<BITS, D> even, odd;
+  if constexpr (BITS == 4) even.or_bits = odd.or_bits = q4_or_bits();
   auto send = [&](WalkUnit<BITS, D>& u, int k) {
     if (k != 0 && (k & 31) == 0) ids = fetch_ids(k);
-    u.load(p, kvh, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1), n, g);
+    u.load(base, unit_offsets<BITS>(p, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1)), n, g);
   };
   if (n_mine > 0) send(even, 0);
 
@@ -515,7 +563,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
 // ---------------------------------------------------------------------------------
 // More query rows (drafted tokens, chunks of a prompt): the four waves of a workgroup own NQT tiles of 16 rows each and walk the
 // units together.  Each wave fetches and unpacks a quarter of a unit and puts it into LDS in operand order, so that the
-// unpacking is paid once per workgroup; fetches run two units ahead of their use (one in registers, one in LDS), with
+// unpacking is paid once per workgroup; fetches run three units ahead of their use (two in registers, one in LDS), with
 // one barrier per unit.  A row's softmax state never leaves its wave.
 // ---------------------------------------------------------------------------------
 template <int BITS, int D, int NQT, bool HAS_MASK, int OCC>
@@ -545,20 +593,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
     return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
   };
   int ids = i_begin < i_end ? fetch_ids(i_begin) : 0, ids_first = i_begin;
-  UnitShare<BITS, D> share;
-  auto send = [&](int i) {
+  const LaneBase base = UnitShare<BITS, D>::base(p, kvh, wave, n, g);
+  const uint32_t or_bits = q4_or_bits();
+  UnitShare<BITS, D> even, odd;
+  auto send = [&](UnitShare<BITS, D>& share, int i) {
+    if (i >= i_end) return;
     if (i - ids_first == 32) ids = fetch_ids(i), ids_first = i;
-    share.load(p, kvh, __builtin_amdgcn_readlane(ids, 2 * (i - ids_first)), __builtin_amdgcn_readlane(ids, 2 * (i - ids_first) + 1), wave, n, g);
+    share.load(base, unit_offsets<BITS>(p, __builtin_amdgcn_readlane(ids, 2 * (i - ids_first)), __builtin_amdgcn_readlane(ids, 2 * (i - ids_first) + 1)),
+               wave, n, g);
   };
-  auto put = [&](int i) {
+  auto put = [&](UnitShare<BITS, D>& share, int i) {
+    if (i >= i_end) return;
     u32x4 keep = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
     if (BITS == 16) {
       const int t0 = 32 * walk.unit(i);
       if (t0 < start || t0 + 32 > wg_end || t0 < wg_low) keep = walk_keep(t0, g, start, walk.sink_end, wg_low, wg_end);
     }
-    share.put(stage[(i - i_begin) & 1], wave, lane, keep);
+    share.put(stage[(i - i_begin) & 1], wave, lane, keep, or_bits);
   };
-  if (i_begin < i_end) send(i_begin);
+  send(even, i_begin);
+  send(odd, i_begin + 1);
 
   WalkRows<D, NQT> st;
   const int w_first = r_first + wave * NQT * 16, w_last = min(R, w_first + NQT * 16) - 1;  // this wave's rows
@@ -573,12 +627,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
   const int max_low = p.window > 0 ? len - S + w_last / p.n_rep - p.window + 1 : 0;
   const int row_end = !any_rows ? 0 : (p.causal ? min(len, len - S + w_last / p.n_rep + 1) : len);
 
-  if (i_begin < i_end) put(i_begin);
-  if (i_begin + 1 < i_end) send(i_begin + 1);
+  put(even, i_begin);
+  send(even, i_begin + 2);
   __syncthreads();
-  for (int i = i_begin; i < i_end; ++i) {
-    if (i + 1 < i_end) put(i + 1);  // (every wave has left that stage: the barrier of the turn before)
-    if (i + 2 < i_end) send(i + 2);
+  // One turn: unit i + 1 goes from `next` into the stage that every wave left before the last barrier, `next` fetches unit
+  // i + 3, unit i is used.
+  auto turn = [&](UnitShare<BITS, D>& next, int i) {
+    put(next, i + 1);
+    send(next, i + 3);
     const int t0 = 32 * walk.unit(i);
     if (t0 < row_end && (t0 + 32 > row_low || t0 < walk.sink_end)) {
       MaskRegs<NQT> mregs;
@@ -588,6 +644,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
       walk_unit<BITS, D, NQT, HAS_MASK>(u, st, full, t0, start, walk.sink_end, g, mregs);
     }
     __syncthreads();
+  };
+  for (int i = i_begin; i < i_end; i += 2) {
+    turn(odd, i);
+    if (i + 1 < i_end) turn(even, i + 1);
   }
   walk_finish<D, NQT, HAS_MASK>(st);
 #pragma unroll
