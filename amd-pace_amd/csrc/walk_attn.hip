@@ -185,15 +185,6 @@ struct WalkUnit<4, D> {
   __device__ __forceinline__ void drop(const u32x4&) {}  // (a 4-bit pool holds finite values only)
 };
 
-// A unit in LDS, shared by the waves of a workgroup: operands lane for lane.
-template <int D>
-struct StagedUnit {
-  const u32x4* at;  // this lane's 16 bytes of the first operand
-  __device__ __forceinline__ u32x4 k(int t, int kk) const { return at[(t * (D / 32) + kk) * 64]; }
-  __device__ __forceinline__ u32x4 v(int j) const { return at[(D / 16 + j) * 64]; }
-  __device__ __forceinline__ void drop(const u32x4&) {}
-};
-
 // A wave's quarter of a unit on its way into LDS: KPW of the K operands (tile wave & 1, steps kk0 ..) and VPW of the V operands
 // (dim tiles j0 ..).  Where the operands do not divide by four (head size 96) two waves make the same one.
 template <int BITS, int D>
@@ -272,7 +263,8 @@ template <int D, int NQT>
 struct WalkRows {
   u32x4 q[NQT][D / 32];
   f32x4 o[NQT][D / 16];
-  float m[NQT], m_top[NQT], m_neg[NQT], l[NQT];  // see RowState
+  f32x4 sum[NQT];                        // the weights' sum, four times over (a product with ones)
+  float m[NQT], m_top[NQT], m_neg[NQT];  // see RowState
   float c[NQT];    // score product -> log2 units
   float cn[NQT];   // score product -> natural units (with a mask tensor)
   int limit[NQT];  // last readable token (-1: no such row, or none)
@@ -332,7 +324,7 @@ __device__ __forceinline__ int walk_row(const WalkParams& p, WalkRows<D, NQT>& s
   const float down = __uint_as_float((uint32_t)(127 - up) << 23);
   st.cn[qt] = p.scale * down;
   st.c[qt] = fminf(fmaxf(p.scale_log2 * down, 0x1p-126f), 0x1p126f);  // (not 0 or infinite: it multiplies -inf and 0)
-  st.m[qt] = kNegInf, st.m_top[qt] = kNegInf, st.m_neg[qt] = 0.f, st.l[qt] = 0.f;
+  st.m[qt] = kNegInf, st.m_top[qt] = kNegInf, st.m_neg[qt] = 0.f, st.sum[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) st.o[qt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   return valid ? st.limit[qt] : 0x7fffffff;
@@ -350,23 +342,26 @@ __device__ __forceinline__ u32x4 walk_keep(int t0, int g, int start, int sink_en
   return keep;
 }
 
-// One unit against the rows of a wave.  full (wave-uniform): every row reads all of its 32 tokens.
-template <int BITS, int D, int NQT, bool HAS_MASK, class Unit>
-__device__ __forceinline__ void walk_unit(const Unit& u, WalkRows<D, NQT>& st, bool full, int t0, int start, int sink_end, int g,
-                                          const MaskRegs<NQT>& mregs) {
-#pragma clang fp contract(off)
-  constexpr int KK = D / 32, MT = D / 16;
-  f32x4 sc[NQT][2];
+// One unit against the rows of a wave, in three steps.  First the scores.
+template <int BITS, int D, int NQT, class K>
+__device__ __forceinline__ void walk_scores(K&& k, const WalkRows<D, NQT>& st, f32x4 (&sc)[NQT][2]) {
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt) sc[qt][0] = sc[qt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const u32x4 k = u.k(t, kk);
+    for (int kk = 0; kk < D / 32; ++kk) {
+      const u32x4 a = k(t, kk);
 #pragma unroll
-      for (int qt = 0; qt < NQT; ++qt) sc[qt][t] = walk_mfma<BITS>(k, st.q[qt][kk], sc[qt][t]);
+      for (int qt = 0; qt < NQT; ++qt) sc[qt][t] = walk_mfma<BITS>(a, st.q[qt][kk], sc[qt][t]);
     }
+}
+
+// Scores -> weights (operands of the second product).  full (wave-uniform): every row reads all of the unit's 32 tokens.
+template <int BITS, int D, int NQT, bool HAS_MASK>
+__device__ __forceinline__ void walk_weights(f32x4 (&sc)[NQT][2], WalkRows<D, NQT>& st, u32x4 (&pb)[NQT], bool full, int t0, int start, int sink_end,
+                                             int g, const MaskRegs<NQT>& mregs) {
+#pragma clang fp contract(off)
   if (HAS_MASK) {
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt)
@@ -383,14 +378,16 @@ __device__ __forceinline__ void walk_unit(const Unit& u, WalkRows<D, NQT>& st, b
         sc[qt][e >> 2][e & 3] = (e > hi) | (e < lo) | ((e < wl) & (e >= se)) ? kNegInf : sc[qt][e >> 2][e & 3];  // whatever the token holds
     }
   }
-  u32x4 pb[NQT];
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt) {
     float s[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = sc[qt][e >> 2][e & 3];
     const float c = HAS_MASK ? kLog2e : st.c[qt];
-    const float mine = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    // (this maximum hands NaN on, which needs no instruction to quiet its operands; a row with a NaN weight is NaN throughout)
+    float mine = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mine = __builtin_elementwise_maximum(mine, s[e]);
     if (__any(mine > st.m_top[qt])) {  // the reference follows the maximum lazily, as in softmax_and_output
       const float mx = row_max4(mine);
       const float m_old = st.m[qt], m_new = fmaxf(m_old, mx);
@@ -399,46 +396,47 @@ __device__ __forceinline__ void walk_unit(const Unit& u, WalkRows<D, NQT>& st, b
       st.m[qt] = m_new;
       st.m_top[qt] = m_new + kLazyLog2 / c;
       st.m_neg[qt] = kWeightShift<BITS> - m_use * c;
-      st.l[qt] *= alpha;
+      st.sum[qt][0] *= alpha;
 #pragma unroll
-      for (int j = 0; j < MT; ++j) st.o[qt][j] *= alpha;
+      for (int j = 0; j < D / 16; ++j) st.o[qt][j] *= alpha;
     }
-    float w[8], sum = 0.f;
+    float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, st.m_neg[qt]));
-      sum += w[e];
-    }
-    st.l[qt] += sum;
+    for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, st.m_neg[qt]));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (BITS == 4) pb[qt][i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)w[2 * i], (_Float16)w[2 * i + 1]});
       else pb[qt][i] = pack_bf16x2(w[2 * i], w[2 * i + 1]);
     }
   }
+}
+
+// The second product.  The weights are summed by the matrix cores too, as rounded: the same weights then stand above and below the
+// fraction, and eight additions per tile are saved where the vector unit is the bound.
+template <int BITS, int D, int NQT, class V>
+__device__ __forceinline__ void walk_output(V&& v, WalkRows<D, NQT>& st, const u32x4 (&pb)[NQT]) {
+  const uint32_t one2 = BITS == 4 ? 0x3c003c00u : 0x3f803f80u;
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const u32x4 v = u.v(j);
+  for (int qt = 0; qt < NQT; ++qt) st.sum[qt] = walk_mfma<BITS>(u32x4{one2, one2, one2, one2}, pb[qt], st.sum[qt]);
 #pragma unroll
-    for (int qt = 0; qt < NQT; ++qt) st.o[qt][j] = walk_mfma<BITS>(v, pb[qt], st.o[qt][j]);
+  for (int j = 0; j < D / 16; ++j) {
+    const u32x4 a = v(j);
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) st.o[qt][j] = walk_mfma<BITS>(a, pb[qt], st.o[qt][j]);
   }
 }
 
-// Row sums over the four lanes of a row, running maximum in log2 units (-inf stays -inf).
+// Running maximum in log2 units (-inf stays -inf).
 template <int D, int NQT, bool HAS_MASK>
 __device__ __forceinline__ void walk_finish(WalkRows<D, NQT>& st) {
 #pragma unroll
-  for (int qt = 0; qt < NQT; ++qt) {
-    st.l[qt] += xor_lanes(st.l[qt], 16);
-    st.l[qt] += xor_lanes(st.l[qt], 32);
-    st.m[qt] *= HAS_MASK ? kLog2e : st.c[qt];
-  }
+  for (int qt = 0; qt < NQT; ++qt) st.m[qt] *= HAS_MASK ? kLog2e : st.c[qt];
 }
 
 // A finished row: the output, or this partition's share of it.
 template <int D, int NQT>
 __device__ __forceinline__ void walk_store(const WalkParams& p, const WalkRows<D, NQT>& st, int qt, int b, int part, int g) {
-  const float l = st.l[qt];
+  const float l = st.sum[qt][0];
   if (p.max_parts == 1) {
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that read nothing is 0; NaN stays NaN
     uint16_t* op = p.out + (int64_t)b * p.o_sb + (int64_t)st.hq[qt] * p.o_sh + (int64_t)st.s[qt] * p.o_ss + 4 * g;
@@ -483,6 +481,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const WalkItem at = walk_item(p);
   const int b = at.b, kvh = at.kvh, part = at.part;
+  const int32_t* row = p.table + (int64_t)b * p.table_stride;
+  // Without a window and padding the units do not depend on the length: the first block ids are asked for along with it.
+  const bool known = p.window == 0 && p.kv_start == nullptr;
+  int early = 0;
+  if (known) {
+    const int t = 2 * (part * p.part_units + wave + NW * (lane >> 1)) + (lane & 1);
+    early = t < p.table_stride ? row[t] : 0;
+  }
   const int len = walk_len(p, b), start = walk_start(p, b, len);
   const int S = p.q_len, R = S * p.n_rep;
   const Walk walk = walk_of(p, len, start, 0, S - 1);
@@ -492,19 +498,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
   const int n_mine = i_end - i_begin > wave ? (i_end - i_begin - wave + NW - 1) / NW : 0;
 
   // Pool block ids of 32 units of this wave, one per lane; never outside the pool, whatever the table holds.
-  const int32_t* row = p.table + (int64_t)b * p.table_stride;
+  auto inside = [&](int id) { return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id); };
   auto fetch_ids = [&](int first) {
     const int i = i_begin + wave + NW * (first + (lane >> 1));
     const int t = 2 * walk.unit(i) + (lane & 1);
-    const int id = i < i_end && t < p.table_stride ? row[t] : 0;
-    return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
+    return inside(i < i_end && t < p.table_stride ? row[t] : 0);
   };
-  int ids = n_mine > 0 ? fetch_ids(0) : 0;
+  int ids = known ? inside(early) : (n_mine > 0 ? fetch_ids(0) : 0);
   const LaneBase base = WalkUnit<BITS, D>::base(p, kvh, n, g);
+  constexpr bool TWO = !(BITS == 16 && D == 256);  // registers for a second unit under way
   WalkUnit<BITS, D> even, odd;
   if constexpr (BITS == 4) even.or_bits = odd.or_bits = q4_or_bits();
   auto send = [&](WalkUnit<BITS, D>& u, int k) {
-    if (k != 0 && (k & 31) == 0) ids = fetch_ids(k);
     u.load(base, unit_offsets<BITS>(p, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1)), n, g);
   };
   if (n_mine > 0) send(even, 0);
@@ -523,13 +528,42 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     if (HAS_MASK) load_mask_regs<1>(mregs, p, st.mask_off, t0, g);
     const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
     if (BITS == 16 && !full) u.drop(walk_keep(t0, g, start, walk.sink_end, row_low, len));
-    walk_unit<BITS, D, 1, HAS_MASK>(u, st, full, t0, start, walk.sink_end, g, mregs);
+    f32x4 sc[1][2];
+    u32x4 pb[1];
+    walk_scores<BITS, D, 1>([&](int t, int kk) { return u.k(t, kk); }, st, sc);
+    walk_weights<BITS, D, 1, HAS_MASK>(sc, st, pb, full, t0, start, walk.sink_end, g, mregs);
+    walk_output<BITS, D, 1>([&](int j) { return u.v(j); }, st, pb);
   };
-  for (int k = 0; k < n_mine; k += 2) {
-    if (k + 1 < n_mine) send(odd, k + 1);
-    take(even, k);
-    if (k + 2 < n_mine) send(even, k + 2);
-    if (k + 1 < n_mine) take(odd, k + 1);
+  // 32 units per set of block ids.  (Every turn of the inner loop fetches: behind a fetch that may or may not have been sent, the
+  // compiler would have the wave wait for all that is under way before it uses the unit before it.)
+  for (int k0 = 0; k0 < n_mine; k0 += 32) {
+    const int k1 = min(k0 + 32, n_mine);
+    if (k0 > 0) {
+      ids = fetch_ids(k0);
+      send(even, k0);
+    }
+    int k = k0;
+    if constexpr (TWO) {
+      for (; k + 2 < k1; k += 2) {
+        send(odd, k + 1);
+        take(even, k);
+        send(even, k + 2);
+        take(odd, k + 1);
+      }
+      if (k + 1 < k1) {
+        send(odd, k + 1);
+        take(even, k);
+        take(odd, k + 1);
+      } else {
+        take(even, k);
+      }
+    } else {
+      for (; k + 1 < k1; ++k) {
+        take(even, k);
+        send(even, k + 1);
+      }
+      take(even, k);
+    }
   }
   walk_finish<D, 1, HAS_MASK>(st);
   // Pairwise merge of the waves' states (fixed order: the same bits from call to call).
@@ -542,7 +576,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
       for (int j = 0; j < MT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) slot[16 * j + 4 * g + i] = st.o[0][j][i];
-      if (g == 0) slot[D] = st.m[0], slot[D + 1] = st.l[0];
+      if (g == 0) slot[D] = st.m[0], slot[D + 1] = st.sum[0][0];
     }
     __syncthreads();
     if (receiver) {
@@ -552,7 +586,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
       for (int j = 0; j < MT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) st.o[0][j][i] = st.o[0][j][i] * wa + slot[16 * j + 4 * g + i] * wb;
-      st.l[0] = st.l[0] * wa + l_b * wb;
+      st.sum[0][0] = st.sum[0][0] * wa + l_b * wb;
       st.m[0] = m_new;
     }
     __syncthreads();
@@ -568,7 +602,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
 // ---------------------------------------------------------------------------------
 template <int BITS, int D, int NQT, bool HAS_MASK, int OCC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) void walk_rows_kernel(const WalkParams p) {
-  constexpr int OPERANDS = D / 8;  // of a unit, 16 bytes per lane each
+  constexpr int KK = D / 32, MT = D / 16, OPERANDS = 2 * MT;  // operands of a unit: K's, then V's, 16 bytes per lane each
   __shared__ __attribute__((aligned(16))) u32x4 stage[2][OPERANDS * 64];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -586,33 +620,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
   const int wg_end = p.causal ? min(len, len - S + s_last + 1) : len;
 
   const int32_t* row = p.table + (int64_t)b * p.table_stride;
-  auto fetch_ids = [&](int first) {  // pool blocks of units first .. first + 31, one per lane; never outside the pool
-    const int i = first + (lane >> 1);
+  // Pool blocks of 64 units from c0 on, one per lane in each of two registers; never outside the pool.
+  auto fetch_id = [&](int i) {
     const int t = 2 * walk.unit(i) + (lane & 1);
     const int id = i < i_end && t < p.table_stride ? row[t] : 0;
     return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
   };
-  int ids = i_begin < i_end ? fetch_ids(i_begin) : 0, ids_first = i_begin;
+  int c0 = i_begin, ids_lo = fetch_id(c0 + (lane >> 1)), ids_hi = fetch_id(c0 + 32 + (lane >> 1));
   const LaneBase base = UnitShare<BITS, D>::base(p, kvh, wave, n, g);
   const uint32_t or_bits = q4_or_bits();
   UnitShare<BITS, D> even, odd;
   auto send = [&](UnitShare<BITS, D>& share, int i) {
-    if (i >= i_end) return;
-    if (i - ids_first == 32) ids = fetch_ids(i), ids_first = i;
-    share.load(base, unit_offsets<BITS>(p, __builtin_amdgcn_readlane(ids, 2 * (i - ids_first)), __builtin_amdgcn_readlane(ids, 2 * (i - ids_first) + 1)),
-               wave, n, g);
+    const int at = 2 * (i - c0);  // (past the 64 units: whatever block the lane holds; nobody reads that share)
+    const int idA = at & 64 ? __builtin_amdgcn_readlane(ids_hi, at & 63) : __builtin_amdgcn_readlane(ids_lo, at & 63);
+    const int idB = at & 64 ? __builtin_amdgcn_readlane(ids_hi, (at & 63) + 1) : __builtin_amdgcn_readlane(ids_lo, (at & 63) + 1);
+    share.load(base, unit_offsets<BITS>(p, idA, idB), wave, n, g);
   };
-  auto put = [&](UnitShare<BITS, D>& share, int i) {
-    if (i >= i_end) return;
+  auto put = [&](UnitShare<BITS, D>& share, int i) {  // (past the last unit: whatever the share holds, into a stage nobody reads)
     u32x4 keep = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
     if (BITS == 16) {
       const int t0 = 32 * walk.unit(i);
       if (t0 < start || t0 + 32 > wg_end || t0 < wg_low) keep = walk_keep(t0, g, start, walk.sink_end, wg_low, wg_end);
     }
-    share.put(stage[(i - i_begin) & 1], wave, lane, keep, or_bits);
+    share.put(stage[(i - c0) & 1], wave, lane, keep, or_bits);
   };
-  send(even, i_begin);
-  send(odd, i_begin + 1);
+  send(even, c0);
+  send(odd, c0 + 1);
 
   WalkRows<D, NQT> st;
   const int w_first = r_first + wave * NQT * 16, w_last = min(R, w_first + NQT * 16) - 1;  // this wave's rows
@@ -627,27 +660,59 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
   const int max_low = p.window > 0 ? len - S + w_last / p.n_rep - p.window + 1 : 0;
   const int row_end = !any_rows ? 0 : (p.causal ? min(len, len - S + w_last / p.n_rep + 1) : len);
 
-  put(even, i_begin);
-  send(even, i_begin + 2);
-  __syncthreads();
-  // One turn: unit i + 1 goes from `next` into the stage that every wave left before the last barrier, `next` fetches unit
-  // i + 3, unit i is used.
+  // One turn: unit i + 1 of the set goes from `next` into LDS, `next` fetches unit i + 3, unit i is used.  With two tiles per wave LDS
+  // reads travel behind vector work: the K operands are asked for before the unpacking, the V operands before the softmax
+  // that needs them after it.  (With one tile a third workgroup on the compute unit does that, and registers are kept for
+  // it; head size 256 and a mask have none to spare.)  At the barrier every wave has taken what it needs of unit i, and every share of
+  // unit i + 1 is in place.
+  constexpr bool AHEAD = D <= 128 && NQT == 2 && !HAS_MASK;
   auto turn = [&](UnitShare<BITS, D>& next, int i) {
+    const int t0 = 32 * walk.unit(i);
+    const u32x4* unit = &stage[(i - c0) & 1][lane];
+    u32x4 kop[AHEAD ? 2 : 1][AHEAD ? KK : 1], vop[AHEAD ? MT : 1];
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) kop[t][kk] = unit[(t * KK + kk) * 64];
+    }
     put(next, i + 1);
     send(next, i + 3);
-    const int t0 = 32 * walk.unit(i);
     if (t0 < row_end && (t0 + 32 > row_low || t0 < walk.sink_end)) {
       MaskRegs<NQT> mregs;
       if (HAS_MASK) load_mask_regs<NQT>(mregs, p, st.mask_off, t0, g);
       const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
-      const StagedUnit<D> u = {&stage[(i - i_begin) & 1][lane]};
-      walk_unit<BITS, D, NQT, HAS_MASK>(u, st, full, t0, start, walk.sink_end, g, mregs);
+      f32x4 sc[NQT][2];
+      u32x4 pb[NQT];
+      walk_scores<BITS, D, NQT>([&](int t, int kk) { return AHEAD ? kop[AHEAD ? t : 0][AHEAD ? kk : 0] : unit[(t * KK + kk) * 64]; }, st, sc);
+      if constexpr (AHEAD) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j) vop[j] = unit[(MT + j) * 64];
+      }
+      walk_weights<BITS, D, NQT, HAS_MASK>(sc, st, pb, full, t0, start, walk.sink_end, g, mregs);
+      walk_output<BITS, D, NQT>([&](int j) { return AHEAD ? vop[AHEAD ? j : 0] : unit[(MT + j) * 64]; }, st, pb);
     }
     __syncthreads();
   };
-  for (int i = i_begin; i < i_end; i += 2) {
-    turn(odd, i);
-    if (i + 1 < i_end) turn(even, i + 1);
+  // 64 units per set of block ids.  (Every turn of the inner loop fetches, past the last unit block 0 of the pool, which nobody reads:
+  // behind a fetch that may or may not have been sent, the compiler would have the wave wait for all that is under way
+  // before it uses the share before it.)
+  for (; c0 < i_end; c0 += 64) {
+    if (c0 > i_begin) {
+      ids_lo = fetch_id(c0 + (lane >> 1)), ids_hi = fetch_id(c0 + 32 + (lane >> 1));
+      send(even, c0);
+      send(odd, c0 + 1);
+    }
+    const int c1 = min(c0 + 64, i_end);
+    put(even, c0);
+    send(even, c0 + 2);
+    __syncthreads();
+    int i = c0;
+    for (; i + 1 < c1; i += 2) {
+      turn(odd, i);
+      turn(even, i + 1);
+    }
+    if (i < c1) turn(odd, i);
   }
   walk_finish<D, NQT, HAS_MASK>(st);
 #pragma unroll
@@ -655,50 +720,78 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
     if (w_first + qt * 16 + n < R) walk_store(p, st, qt, b, part, g);
 }
 
-// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partitions of a query row, one wave per row.  A lane fetches the
-// (maximum, sum) pair of one partition, and owns the dims 2 lane, 2 lane + 1 (+ 128).
-template <int D>
-__global__ __launch_bounds__(64) void walk_merge_kernel(const WalkParams p, int32_t rows_per_group) {
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partitions of a query row.  A wave takes eight partitions at a time, a
+// lane the dims 2 lane, 2 lane + 1 (+ 128); WPR waves share a row (partitions in turn, joined through LDS).  The launch is a
+// chain of memory round trips, so the first eight partials are fetched before the sequence's length says how many there
+// are: the workspace holds max_parts of every row, and what is not a partial is not used.
+template <int D, int WPR>
+__global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int32_t rows_per_group, int32_t total_rows) {
   constexpr int PASSES = (D + 127) / 128;
-  const int64_t row = blockIdx.x;  // (b, hq, s)
-  const int S = p.q_len, s = (int)(row % S), hq = (int)(row / S % p.num_q_heads), b = (int)(row / S / p.num_q_heads), lane = threadIdx.x;
-  const int len = walk_len(p, b), start = walk_start(p, b, len);
-  const int r = s * p.n_rep + hq % p.n_rep, r_first = r / rows_per_group * rows_per_group;
-  const Walk walk = walk_of(p, len, start, r_first / p.n_rep, (min(S * p.n_rep, r_first + rows_per_group) - 1) / p.n_rep);
-  const int n_parts = walk_parts(p, walk.total);
+  __shared__ float join[WPR > 1 ? WPR : 1][2 * PASSES + 2][WPR > 1 ? 64 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave % WPR;
+  const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;  // (b, hq, s)
+  if (row >= total_rows) return;  // (WPR == 1 only: whole waves; else the grid is exact)
+  const int S = p.q_len, s = (int)(row % S), hq = (int)(row / S % p.num_q_heads), b = (int)(row / S / p.num_q_heads);
   const float* ml = p.part_ml + row * p.max_parts * 2;
   const float* po = p.part_o + row * p.max_parts * D;
-  float M = kNegInf;
-  for (int base = 0; base < n_parts; base += 64) M = fmaxf(M, base + lane < n_parts ? ml[2 * (base + lane)] : kNegInf);
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) M = fmaxf(M, __shfl_xor(M, o, 64));
-  const float m_use = M == kNegInf ? 0.f : M;
-  float acc[PASSES][2], L = 0.f;
+  const int d0 = 2 * lane;
+  float acc[PASSES][2], M = kNegInf, L = 0.f;
 #pragma unroll
   for (int e = 0; e < PASSES; ++e) acc[e][0] = acc[e][1] = 0.f;
-  const int d0 = 2 * lane;
-  for (int base = 0; base < n_parts; base += 64) {
-    const bool mine = base + lane < n_parts;
-    const float w_mine = mine ? __builtin_amdgcn_exp2f(ml[2 * (base + lane)] - m_use) : 0.f, l_mine = mine ? ml[2 * (base + lane) + 1] : 0.f;
-    const int here = min(64, n_parts - base);
-    for (int j0 = 0; j0 < here; j0 += 8) {
-      u32x2 v[8][PASSES];
+  int n_parts = p.max_parts;
+  for (int base = 8 * slice; base < n_parts; base += 8 * WPR) {
+    const int mine = min(base + (lane & 7), p.max_parts - 1);
+    const u32x2 pair = *reinterpret_cast<const u32x2*>(ml + 2 * mine);
+    u32x2 v[8][PASSES];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int e = 0; e < PASSES; ++e) {
-          v[j][e] = u32x2{0u, 0u};
-          if (j0 + j < here && d0 + 128 * e < D) v[j][e] = *reinterpret_cast<const u32x2*>(po + (int64_t)(base + j0 + j) * D + d0 + 128 * e);
-        }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j0 + j < here) {
-          const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_mine), j0 + j));
-          L += w * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l_mine), j0 + j));
-#pragma unroll
-          for (int e = 0; e < PASSES; ++e) acc[e][0] += w * __uint_as_float(v[j][e][0]), acc[e][1] += w * __uint_as_float(v[j][e][1]);
-        }
+      for (int e = 0; e < PASSES; ++e) {
+        v[j][e] = u32x2{0u, 0u};
+        if (base + j < p.max_parts && d0 + 128 * e < D) v[j][e] = *reinterpret_cast<const u32x2*>(po + (int64_t)(base + j) * D + d0 + 128 * e);
       }
+    if (base == 8 * slice) {
+      const int len = walk_len(p, b), start = walk_start(p, b, len);
+      const int r = s * p.n_rep + hq % p.n_rep, r_first = r / rows_per_group * rows_per_group;
+      n_parts = walk_parts(p, walk_of(p, len, start, r_first / p.n_rep, (min(S * p.n_rep, r_first + rows_per_group) - 1) / p.n_rep).total);
+    }
+    float m_mine = base + (lane & 7) < n_parts ? __uint_as_float(pair[0]) : kNegInf;
+    float top = m_mine;
+    top = fmaxf(top, __shfl_xor(top, 1, 64)), top = fmaxf(top, __shfl_xor(top, 2, 64)), top = fmaxf(top, __shfl_xor(top, 4, 64));
+    const float M_new = fmaxf(M, top), m_use = M_new == kNegInf ? 0.f : M_new, old = __builtin_amdgcn_exp2f(M - m_use);
+    const float w_mine = __builtin_amdgcn_exp2f(m_mine - m_use);
+    M = M_new, L *= old;
+#pragma unroll
+    for (int e = 0; e < PASSES; ++e) acc[e][0] *= old, acc[e][1] *= old;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (base + j < n_parts) {  // wave-uniform
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_mine), j));
+        L += w * __uint_as_float(__builtin_amdgcn_readlane(pair[1], j));
+#pragma unroll
+        for (int e = 0; e < PASSES; ++e) acc[e][0] += w * __uint_as_float(v[j][e][0]), acc[e][1] += w * __uint_as_float(v[j][e][1]);
+      }
+    }
+  }
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int e = 0; e < PASSES; ++e) join[slice][2 * e][lane] = acc[e][0], join[slice][2 * e + 1][lane] = acc[e][1];
+    join[slice][2 * PASSES][lane] = M, join[slice][2 * PASSES + 1][lane] = L;
+    __syncthreads();
+    if (slice != 0) return;
+    float all = kNegInf;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) all = fmaxf(all, join[w][2 * PASSES][lane]);
+    const float m_use = all == kNegInf ? 0.f : all;
+    L = 0.f;
+#pragma unroll
+    for (int e = 0; e < PASSES; ++e) acc[e][0] = acc[e][1] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      const float f = __builtin_amdgcn_exp2f(join[w][2 * PASSES][lane] - m_use);
+      L += f * join[w][2 * PASSES + 1][lane];
+#pragma unroll
+      for (int e = 0; e < PASSES; ++e) acc[e][0] += f * join[w][2 * e][lane], acc[e][1] += f * join[w][2 * e + 1][lane];
     }
   }
   const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
@@ -732,13 +825,22 @@ static WalkShape walk_shape(const pace_kv_pool_t* pool, const pace_paged_attn_ar
   if (a->window > 0) units = std::min(units, ((int64_t)a->window + a->q_len) / 32 + 2 + a->sinks / 32 + 2);
   units = std::max<int64_t>(units, 1);
   const int64_t at_once = s.nqt == 0 ? walk_waves(D) : 1;  // units a workgroup works on side by side
-  const int64_t per_cu = s.nqt == 0 ? 4 * walk_occ(D) / walk_waves(D) : rows_occ(D, s.nqt);
-  const int64_t groups = (int64_t)a->batch * pool->num_kv_heads * s.n_qgroups, slots = compute_units() * per_cu;
-  // Enough workgroups to fill the GPU once, at least four units each, and 4096 tokens at most, so that one long sequence
-  // among short ones is shared out.
-  int64_t per = a->partition_tokens > 0 ? a->partition_tokens / 32 : std::min<int64_t>(std::max<int64_t>(units * groups / slots, 4), 128);
+  const int64_t groups = (int64_t)a->batch * pool->num_kv_heads * s.n_qgroups, cus = compute_units();
+  int64_t per = a->partition_tokens / 32, parts;
+  if (per == 0) {
+    // How many workgroups share a sequence.  One per compute unit is enough for walk_attn_kernel, whose waves fetch ahead; the
+    // others want as many as fit side by side, and twice that with few rows, where lengths may differ (a batch of drafts)
+    // and partial results are small.  A cut costs a second launch and a trip of the partial results: no share below
+    // min_share units for that.  Lengths are not known here, so a sequence that could be far longer than the others is cut
+    // at about 4096 tokens.
+    const int64_t want = s.nqt == 0 ? cus : cus * rows_occ(D, s.nqt) * (s.nqt == 1 && rows <= 64 ? 2 : 1);
+    const int64_t min_share = s.nqt == 0 ? 4 : 12;
+    parts = std::max<int64_t>((units + 64) / 128, groups >= want ? 1 : (want + groups - 1) / groups);
+    parts = std::max<int64_t>(std::min(parts, units / min_share), 1);
+    per = (units + parts - 1) / parts;
+  }
   per = (std::max<int64_t>(per, 1) + at_once - 1) / at_once * at_once;
-  int64_t parts = (units + per - 1) / per;
+  parts = (units + per - 1) / per;
   const size_t one = (size_t)a->batch * a->num_q_heads * a->q_len * (D + 2) * sizeof(float);
   if (parts > 1 && workspace_bytes / one < (size_t)parts) {
     parts = std::max<int64_t>((int64_t)(workspace_bytes / one), 1);
@@ -810,7 +912,10 @@ int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, con
     } else {
       if (masked) launch_walk_kernel<16, D, true>(p, sh.nqt, stream); else launch_walk_kernel<16, D, false>(p, sh.nqt, stream);
     }
-    if (sh.max_parts > 1) hipLaunchKernelGGL(walk_merge_kernel<D>, dim3((unsigned)rows), dim3(64), 0, stream, p, sh.group_rows);
+    if (sh.max_parts > 8)
+      hipLaunchKernelGGL((walk_merge_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, p, sh.group_rows, (int32_t)rows);
+    else if (sh.max_parts > 1)
+      hipLaunchKernelGGL((walk_merge_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p, sh.group_rows, (int32_t)rows);
   });
   PACE_HIP_CHECK(hipGetLastError());
   return PACE_KV_OK;
