@@ -23,7 +23,14 @@ namespace pace_kv {
 
 struct WalkParams : PagedAttnParams {
   int32_t window, sinks;  // 0: off
-  int32_t part_units;     // 32-token units per workgroup
+  int32_t group_rows;     // query rows of a group
+  // How the groups (sequence, run of query rows) are dealt to workgroups.  shares == 0: one workgroup per group and KV head.  Else
+  // the units of all groups of a KV head lie end to end and `shares` workgroups take equal runs of them (at least
+  // min_share and part_units, a multiple of min_share), so that a batch of any lengths keeps every
+  // workgroup busy for the same time.  A group that one workgroup covers alone is finished there; pieces of others
+  // become partial results, two per workgroup at most -- the group it starts in the middle of or with, and the one it
+  // breaks off -- which walk_merge_kernel joins.
+  int32_t shares, min_share, part_units;
 };
 
 // The units a group of rows walks: [su0, su0 + n_sink), then [wu0, wu0 + total - n_sink).
@@ -54,7 +61,69 @@ __device__ __forceinline__ int walk_len(const WalkParams& p, int b) {
   return max(p.seq_lens[b] + p.len_bias + (p.len_bias_dev ? *p.len_bias_dev : 0), 0);
 }
 __device__ __forceinline__ int walk_start(const WalkParams& p, int b, int len) { return p.kv_start ? min(max(p.kv_start[b], 0), len) : 0; }
-__device__ __forceinline__ int walk_parts(const WalkParams& p, int total) { return min(max((total + p.part_units - 1) / p.part_units, 1), p.max_parts); }
+
+// Group j: sequence j / n_qgroups, its row groups from the last to the first (under the causal limit later rows read more, and the
+// longest workgroups should not be the last to start).
+struct Group {
+  int b, r_first, r_last, s_first, s_last, len, start;
+  Walk walk;
+};
+__device__ __forceinline__ Group walk_group(const WalkParams& p, int j) {
+  Group x;
+  x.b = j / p.n_qgroups;
+  const int qg = p.n_qgroups - 1 - (j - x.b * p.n_qgroups);
+  x.r_first = qg * p.group_rows, x.r_last = min(p.q_len * p.n_rep, x.r_first + p.group_rows) - 1;
+  x.s_first = x.r_first / p.n_rep, x.s_last = x.r_last / p.n_rep;
+  x.len = walk_len(p, x.b), x.start = walk_start(p, x.b, x.len);
+  x.walk = walk_of(p, x.len, x.start, x.s_first, x.s_last);
+  return x;
+}
+
+// Where groups lie in the run of all units: a wave's prefix sums over the groups, 64 at a time.
+struct Shares {
+  int total, share;
+};
+__device__ __forceinline__ int walk_share(const WalkParams& p, int total) {
+  const int share = max(max((total + p.shares - 1) / p.shares, p.min_share), p.part_units);
+  return (share + p.min_share - 1) / p.min_share * p.min_share;
+}
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) v += __shfl_xor(v, o, 64);
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int group_units(const WalkParams& p, int j) { return j < p.batch * p.n_qgroups ? walk_group(p, j).walk.total : 0; }
+__device__ __forceinline__ Shares walk_shares(const WalkParams& p, int lane) {
+  const int n = p.batch * p.n_qgroups;
+  int mine = 0;
+#pragma unroll 4
+  for (int j = lane; j < n; j += 64) mine += group_units(p, j);
+  Shares s;
+  s.total = wave_sum(mine);
+  s.share = walk_share(p, s.total);
+  return s;
+}
+// The group that unit `at` of the run (at < total) lies in, and its place there.
+__device__ __forceinline__ void walk_find(const WalkParams& p, int at, int lane, int& j, int& off) {
+  int before = 0;
+  for (int base = 0;; base += 64) {
+    const int units = group_units(p, base + lane);
+    int upto = units;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int v = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += v;
+    }
+    const uint64_t hit = __ballot(before + upto > at);
+    if (hit != 0 || base + 64 >= p.batch * p.n_qgroups) {
+      const int l = hit != 0 ? __builtin_ctzll(hit) : 63;
+      j = base + l;
+      off = at - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(units, l));
+      return;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+}
 
 // ---- units of either pool ---------------------------------------------------------------------------------------
 template <int N>
@@ -270,7 +339,6 @@ struct WalkRows {
   int limit[NQT];  // last readable token (-1: no such row, or none)
   int low[NQT];    // with a window: first token of it
   int s[NQT], hq[NQT];  // query token and head
-  int64_t mask_off[NQT];
 };
 
 // Weights of halves are kept a factor 2^7 up: with the lazy reference they then reach 2^15, and keep their eleven bits
@@ -316,10 +384,11 @@ __device__ __forceinline__ int walk_row(const WalkParams& p, WalkRows<D, NQT>& s
   st.s[qt] = s, st.hq[qt] = hq;
   st.limit[qt] = valid ? (p.causal ? pos : len - 1) : -1;
   st.low[qt] = p.window > 0 ? pos - p.window + 1 : 0;
-  st.mask_off[qt] = HAS_MASK ? (int64_t)b * p.m_sb + (int64_t)s * p.m_ss : 0;
   const uint16_t* qp = p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh + (int64_t)s * p.q_ss + 8 * g;
 #pragma unroll
-  for (int kk = 0; kk < D / 32; ++kk) st.q[qt][kk] = valid ? *reinterpret_cast<const u32x4*>(qp + kk * 32) : u32x4{0u, 0u, 0u, 0u};
+  for (int kk = 0; kk < D / 32; ++kk) st.q[qt][kk] = *reinterpret_cast<const u32x4*>(qp + kk * 32);  // (no such row: the first one's, and zeros)
+#pragma unroll
+  for (int kk = 0; kk < D / 32; ++kk) st.q[qt][kk] = valid ? st.q[qt][kk] : u32x4{0u, 0u, 0u, 0u};
   const int up = walk_query<BITS, D>(st.q[qt]);
   const float down = __uint_as_float((uint32_t)(127 - up) << 23);
   st.cn[qt] = p.scale * down;
@@ -328,6 +397,26 @@ __device__ __forceinline__ int walk_row(const WalkParams& p, WalkRows<D, NQT>& s
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) st.o[qt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   return valid ? st.limit[qt] : 0x7fffffff;
+}
+
+// Element offset of the mask line of row r.
+__device__ __forceinline__ int64_t walk_mask_line(const WalkParams& p, int b, int r) {
+  return (int64_t)b * p.m_sb + (int64_t)(r < p.q_len * p.n_rep ? r / p.n_rep : 0) * p.m_ss;
+}
+
+// A unit that cannot change any row of the wave: every mask value in it is at the floor (weight exactly 0 next to a real score) and
+// every row has met a real score.  (Rows that have met floor values only may end as an average and need every unit.)
+template <int D, int NQT>
+__device__ __forceinline__ bool walk_masked_out(const MaskRegs<NQT>& mr, const WalkRows<D, NQT>& st) {
+  bool out = true;
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+    float top = mr.a[qt][0];
+#pragma unroll
+    for (int c = 1; c < 8; ++c) top = __builtin_elementwise_maximum(top, mr.a[qt][c]);
+    out = out && (st.limit[qt] < 0 || (top <= kMaskFloor && st.m[qt] > 0.5f * kMaskFloor));
+  }
+  return __all(out);
 }
 
 // Tokens of the unit at t0 that no row of a group reads (past its end, between the sinks and the window) may hold anything in a
@@ -342,19 +431,26 @@ __device__ __forceinline__ u32x4 walk_keep(int t0, int g, int start, int sink_en
   return keep;
 }
 
-// One unit against the rows of a wave, in three steps.  First the scores.
-template <int BITS, int D, int NQT, class K>
+// One unit against the rows of a wave, in three steps.  First the scores.  CHUNK operands are asked for together, ahead of the
+// products they go into (operands that come from LDS; 1: they are made from registers, in the compiler's own order).
+template <int BITS, int D, int NQT, int CHUNK, class K>
 __device__ __forceinline__ void walk_scores(K&& k, const WalkRows<D, NQT>& st, f32x4 (&sc)[NQT][2]) {
+  constexpr int KK = D / 32;
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt) sc[qt][0] = sc[qt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int c = 0; c < 2 * KK; c += CHUNK) {
+    u32x4 a[CHUNK];
 #pragma unroll
-    for (int kk = 0; kk < D / 32; ++kk) {
-      const u32x4 a = k(t, kk);
+    for (int i = 0; i < CHUNK; ++i)
+      if (c + i < 2 * KK) a[i] = k((c + i) / KK, (c + i) % KK);
+    if (CHUNK > 1) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int qt = 0; qt < NQT; ++qt) sc[qt][t] = walk_mfma<BITS>(a, st.q[qt][kk], sc[qt][t]);
-    }
+    for (int i = 0; i < CHUNK; ++i)
+      if (c + i < 2 * KK)
+#pragma unroll
+        for (int qt = 0; qt < NQT; ++qt) sc[qt][(c + i) / KK] = walk_mfma<BITS>(a[i], st.q[qt][(c + i) % KK], sc[qt][(c + i) / KK]);
+  }
 }
 
 // Scores -> weights (operands of the second product).  full (wave-uniform): every row reads all of the unit's 32 tokens.
@@ -413,16 +509,23 @@ __device__ __forceinline__ void walk_weights(f32x4 (&sc)[NQT][2], WalkRows<D, NQ
 
 // The second product.  The weights are summed by the matrix cores too, as rounded: the same weights then stand above and below the
 // fraction, and eight additions per tile are saved where the vector unit is the bound.
-template <int BITS, int D, int NQT, class V>
+template <int BITS, int D, int NQT, int CHUNK, class V>
 __device__ __forceinline__ void walk_output(V&& v, WalkRows<D, NQT>& st, const u32x4 (&pb)[NQT]) {
   const uint32_t one2 = BITS == 4 ? 0x3c003c00u : 0x3f803f80u;
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt) st.sum[qt] = walk_mfma<BITS>(u32x4{one2, one2, one2, one2}, pb[qt], st.sum[qt]);
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
-    const u32x4 a = v(j);
+  for (int c = 0; c < D / 16; c += CHUNK) {
+    u32x4 a[CHUNK];
 #pragma unroll
-    for (int qt = 0; qt < NQT; ++qt) st.o[qt][j] = walk_mfma<BITS>(a, pb[qt], st.o[qt][j]);
+    for (int i = 0; i < CHUNK; ++i)
+      if (c + i < D / 16) a[i] = v(c + i);
+    if (CHUNK > 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < CHUNK; ++i)
+      if (c + i < D / 16)
+#pragma unroll
+        for (int qt = 0; qt < NQT; ++qt) st.o[qt][c + i] = walk_mfma<BITS>(a[i], pb[qt], st.o[qt][c + i]);
   }
 }
 
@@ -433,11 +536,11 @@ __device__ __forceinline__ void walk_finish(WalkRows<D, NQT>& st) {
   for (int qt = 0; qt < NQT; ++qt) st.m[qt] *= HAS_MASK ? kLog2e : st.c[qt];
 }
 
-// A finished row: the output, or this partition's share of it.
+// A finished row: the output (slot < 0), or a partial result.
 template <int D, int NQT>
-__device__ __forceinline__ void walk_store(const WalkParams& p, const WalkRows<D, NQT>& st, int qt, int b, int part, int g) {
+__device__ __forceinline__ void walk_store(const WalkParams& p, const WalkRows<D, NQT>& st, int qt, int b, int kvh, int slot, int row, int g) {
   const float l = st.sum[qt][0];
-  if (p.max_parts == 1) {
+  if (slot < 0) {
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that read nothing is 0; NaN stays NaN
     uint16_t* op = p.out + (int64_t)b * p.o_sb + (int64_t)st.hq[qt] * p.o_sh + (int64_t)st.s[qt] * p.o_ss + 4 * g;
 #pragma unroll
@@ -446,28 +549,44 @@ __device__ __forceinline__ void walk_store(const WalkParams& p, const WalkRows<D
       *reinterpret_cast<u32x2*>(op + 16 * j) = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
     }
   } else {
-    const int64_t at = (((int64_t)b * p.num_q_heads + st.hq[qt]) * p.q_len + st.s[qt]) * p.max_parts + part;
+    const int64_t at = ((int64_t)slot * p.num_kv_heads + kvh) * p.max_parts + row;  // (max_parts: rows of a slot)
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * j + 4 * g) = st.o[qt][j];
     if (g == 0) *reinterpret_cast<u32x2*>(p.part_ml + 2 * at) = u32x2{__float_as_uint(st.m[qt]), __float_as_uint(l)};
   }
 }
 
-// Which (KV head, partition, row group, sequence) workgroup `item` is: KV head fastest, so that one head's K / V stay in one
-// XCD's L2; row groups from the last to the first, because under the causal limit the later rows read more and the longest
-// workgroups should not be the last to start.
-struct WalkItem {
-  int kvh, part, qg, b;
+// The pieces of groups that a workgroup works on, one after the other (wave-uniform): for (WalkTurns t(...); t.more(); t.next()).
+struct WalkTurns {
+  const WalkParams& p;
+  int kvh, w, j, off, left;
+  bool first;
+  __device__ __forceinline__ WalkTurns(const WalkParams& p_, int lane) : p(p_), off(0), left(0), first(true) {
+    const uint32_t item = blockIdx.x;
+    kvh = (int)(item % (uint32_t)p.num_kv_heads);  // fastest: one head's K / V stay in one XCD's L2
+    w = j = (int)(item / (uint32_t)p.num_kv_heads);
+    if (p.shares == 0) return;
+    j = 0;
+    if (p.part_units > 0 && p.batch * p.n_qgroups == 1) {  // one group: nothing to look up
+      off = w * p.part_units, left = w == p.shares - 1 ? 1 << 30 : p.part_units;  // (the last one: whatever there is)
+      return;
+    }
+    const Shares s = walk_shares(p, lane);
+    const int64_t at = (int64_t)w * s.share;
+    if (at >= s.total) return;
+    left = min(s.share, s.total - (int)at);
+    walk_find(p, (int)at, lane, j, off);
+  }
+  // Units [begin, end) of group `x`; slot: where a partial result goes, -1: the group is covered in whole.
+  __device__ __forceinline__ bool piece(const Group& x, int& begin, int& end, int& slot) {
+    begin = off, end = p.shares == 0 ? x.walk.total : (int)min((int64_t)x.walk.total, (int64_t)off + left);
+    slot = begin == 0 && end == x.walk.total ? -1 : (first ? 2 * w : 2 * w + 1);
+    if (p.shares == 0) return true;
+    const int n = max(end - begin, 0);
+    left -= n, off = 0, first = first && n == 0;
+    return n > 0;
+  }
 };
-__device__ __forceinline__ WalkItem walk_item(const WalkParams& p) {
-  WalkItem w;
-  const uint32_t item = blockIdx.x, rest = item / (uint32_t)p.num_kv_heads;
-  w.kvh = (int)(item % (uint32_t)p.num_kv_heads);
-  w.part = (int)(rest % (uint32_t)p.max_parts);
-  const uint32_t bz = rest / (uint32_t)p.max_parts;
-  w.qg = p.n_qgroups - 1 - (int)(bz % (uint32_t)p.n_qgroups), w.b = (int)(bz / (uint32_t)p.n_qgroups);
-  return w;
-}
 
 // ---------------------------------------------------------------------------------
 // Up to 16 query rows per KV head (decode): every wave walks units of its own.  NW waves split a partition's units (wave w:
@@ -479,22 +598,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
   __shared__ float merge_buf[(NW / 2) * SLOT_F];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const WalkItem at = walk_item(p);
-  const int b = at.b, kvh = at.kvh, part = at.part;
-  const int32_t* row = p.table + (int64_t)b * p.table_stride;
-  // Without a window and padding the units do not depend on the length: the first block ids are asked for along with it.
-  const bool known = p.window == 0 && p.kv_start == nullptr;
+  WalkTurns turns(p, lane);
+  const int kvh = turns.kvh, S = p.q_len, R = S * p.n_rep, n_groups = p.batch * p.n_qgroups;
+  // One sequence without a window and padding: its units do not depend on its length, and the first block ids are asked for
+  // along with that.
+  const bool known = n_groups == 1 && p.window == 0 && p.kv_start == nullptr;
   int early = 0;
   if (known) {
-    const int t = 2 * (part * p.part_units + wave + NW * (lane >> 1)) + (lane & 1);
-    early = t < p.table_stride ? row[t] : 0;
+    const int t = 2 * (turns.off + wave + NW * (lane >> 1)) + (lane & 1);
+    early = t < p.table_stride ? p.table[t] : 0;
   }
-  const int len = walk_len(p, b), start = walk_start(p, b, len);
-  const int S = p.q_len, R = S * p.n_rep;
-  const Walk walk = walk_of(p, len, start, 0, S - 1);
-  const int n_parts = walk_parts(p, walk.total);
-  if (part >= n_parts) return;  // uniform over the workgroup
-  const int i_begin = part * p.part_units, i_end = part == n_parts - 1 ? walk.total : min(i_begin + p.part_units, walk.total);
+  do {
+  const Group x = walk_group(p, turns.j);
+  const int b = x.b, len = x.len, start = x.start;
+  const Walk walk = x.walk;
+  int i_begin, i_end, slot;
+  const bool some = turns.piece(x, i_begin, i_end, slot);
+  ++turns.j;
+  if (!some) continue;  // uniform over the workgroup
+  const int32_t* row = p.table + (int64_t)b * p.table_stride;
   const int n_mine = i_end - i_begin > wave ? (i_end - i_begin - wave + NW - 1) / NW : 0;
 
   // Pool block ids of 32 units of this wave, one per lane; never outside the pool, whatever the table holds.
@@ -506,13 +628,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
   };
   int ids = known ? inside(early) : (n_mine > 0 ? fetch_ids(0) : 0);
   const LaneBase base = WalkUnit<BITS, D>::base(p, kvh, n, g);
-  constexpr bool TWO = !(BITS == 16 && D == 256);  // registers for a second unit under way
+  constexpr bool TWO = !(D == 256 && (BITS == 16 || HAS_MASK));  // registers for a second unit under way
   WalkUnit<BITS, D> even, odd;
+  MaskRaw<1> even_mask, odd_mask;  // mask values travel with the unit, ahead of it
+  const int64_t mask_line[1] = {HAS_MASK ? walk_mask_line(p, b, n) : 0};
   if constexpr (BITS == 4) even.or_bits = odd.or_bits = q4_or_bits();
-  auto send = [&](WalkUnit<BITS, D>& u, int k) {
+  auto send = [&](WalkUnit<BITS, D>& u, MaskRaw<1>& m, int k) {
+    if (HAS_MASK) load_mask_raw<1>(m, p, mask_line, 32 * walk.unit(i_begin + wave + NW * k), g);
     u.load(base, unit_offsets<BITS>(p, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1)), n, g);
   };
-  if (n_mine > 0) send(even, 0);
+  if (n_mine > 0) send(even, even_mask, 0);
 
   WalkRows<D, 1> st;
   int min_limit = walk_row<BITS, D, 1, HAS_MASK>(p, st, 0, b, kvh, len, n, g);
@@ -522,17 +647,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
   const int row_low = p.window > 0 ? len - S - p.window + 1 : 0;  // the first row's window, and the last row's
   const int max_low = p.window > 0 ? len - p.window : 0;
 
-  auto take = [&](WalkUnit<BITS, D>& u, int k) {
+  auto take = [&](WalkUnit<BITS, D>& u, const MaskRaw<1>& m, int k) {
     const int t0 = 32 * walk.unit(i_begin + wave + NW * k);
     MaskRegs<1> mregs;
-    if (HAS_MASK) load_mask_regs<1>(mregs, p, st.mask_off, t0, g);
+    if (HAS_MASK) {
+      mask_regs_from_raw<1>(mregs, m, p);
+      if (walk_masked_out<D, 1>(mregs, st)) return;
+    }
     const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
     if (BITS == 16 && !full) u.drop(walk_keep(t0, g, start, walk.sink_end, row_low, len));
     f32x4 sc[1][2];
     u32x4 pb[1];
-    walk_scores<BITS, D, 1>([&](int t, int kk) { return u.k(t, kk); }, st, sc);
+    walk_scores<BITS, D, 1, 1>([&](int t, int kk) { return u.k(t, kk); }, st, sc);
     walk_weights<BITS, D, 1, HAS_MASK>(sc, st, pb, full, t0, start, walk.sink_end, g, mregs);
-    walk_output<BITS, D, 1>([&](int j) { return u.v(j); }, st, pb);
+    walk_output<BITS, D, 1, 1>([&](int j) { return u.v(j); }, st, pb);
   };
   // 32 units per set of block ids.  (Every turn of the inner loop fetches: behind a fetch that may or may not have been sent, the
   // compiler would have the wave wait for all that is under way before it uses the unit before it.)
@@ -540,29 +668,29 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     const int k1 = min(k0 + 32, n_mine);
     if (k0 > 0) {
       ids = fetch_ids(k0);
-      send(even, k0);
+      send(even, even_mask, k0);
     }
     int k = k0;
     if constexpr (TWO) {
       for (; k + 2 < k1; k += 2) {
-        send(odd, k + 1);
-        take(even, k);
-        send(even, k + 2);
-        take(odd, k + 1);
+        send(odd, odd_mask, k + 1);
+        take(even, even_mask, k);
+        send(even, even_mask, k + 2);
+        take(odd, odd_mask, k + 1);
       }
       if (k + 1 < k1) {
-        send(odd, k + 1);
-        take(even, k);
-        take(odd, k + 1);
+        send(odd, odd_mask, k + 1);
+        take(even, even_mask, k);
+        take(odd, odd_mask, k + 1);
       } else {
-        take(even, k);
+        take(even, even_mask, k);
       }
     } else {
       for (; k + 1 < k1; ++k) {
-        take(even, k);
-        send(even, k + 1);
+        take(even, even_mask, k);
+        send(even, even_mask, k + 1);
       }
-      take(even, k);
+      take(even, even_mask, k);
     }
   }
   walk_finish<D, 1, HAS_MASK>(st);
@@ -591,7 +719,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     }
     __syncthreads();
   }
-  if (wave == 0 && n < R) walk_store(p, st, 0, b, part, g);
+  if (wave == 0 && n < R) walk_store(p, st, 0, b, kvh, slot, n, g);
+  } while (p.shares > 0 && turns.left > 0 && turns.j < n_groups);
 }
 
 // ---------------------------------------------------------------------------------
@@ -606,18 +735,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
   __shared__ __attribute__((aligned(16))) u32x4 stage[2][OPERANDS * 64];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const WalkItem at = walk_item(p);
-  const int b = at.b, kvh = at.kvh, part = at.part;
-  const int len = walk_len(p, b), start = walk_start(p, b, len);
-  const int S = p.q_len, R = S * p.n_rep;
-  const int r_first = at.qg * NQT * 64, r_last = min(R, r_first + NQT * 64) - 1;  // the workgroup's rows
-  const int s_first = r_first / p.n_rep, s_last = r_last / p.n_rep;
-  const Walk walk = walk_of(p, len, start, s_first, s_last);
-  const int n_parts = walk_parts(p, walk.total);
-  if (part >= n_parts) return;  // uniform over the workgroup
-  const int i_begin = part * p.part_units, i_end = part == n_parts - 1 ? walk.total : min(i_begin + p.part_units, walk.total);
-  const int wg_low = p.window > 0 ? len - S + s_first - p.window + 1 : 0;  // what no row of the workgroup reads (see walk_keep)
-  const int wg_end = p.causal ? min(len, len - S + s_last + 1) : len;
+  WalkTurns turns(p, lane);
+  const int kvh = turns.kvh, S = p.q_len, R = S * p.n_rep, n_groups = p.batch * p.n_qgroups;
+  do {
+  const Group x = walk_group(p, turns.j);
+  const int b = x.b, len = x.len, start = x.start, r_first = x.r_first;
+  const Walk walk = x.walk;
+  int i_begin, i_end, slot;
+  const bool some = turns.piece(x, i_begin, i_end, slot);
+  ++turns.j;
+  if (!some) continue;  // uniform over the workgroup
+  const int wg_low = p.window > 0 ? len - S + x.s_first - p.window + 1 : 0;  // what no row of the workgroup reads (see walk_keep)
+  const int wg_end = p.causal ? min(len, len - S + x.s_last + 1) : len;
 
   const int32_t* row = p.table + (int64_t)b * p.table_stride;
   // Pool blocks of 64 units from c0 on, one per lane in each of two registers; never outside the pool.
@@ -666,6 +795,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
   // it; head size 256 and a mask have none to spare.)  At the barrier every wave has taken what it needs of unit i, and every share of
   // unit i + 1 is in place.
   constexpr bool AHEAD = D <= 128 && NQT == 2 && !HAS_MASK;
+  constexpr int CHUNK = AHEAD ? 1 : (NQT == 2 ? 4 : 8);
+  MaskRaw<NQT> coming;  // mask values of the next unit: asked for a turn ahead, before that turn's share
+  int64_t mask_line[NQT];
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) mask_line[qt] = HAS_MASK ? walk_mask_line(p, b, w_first + qt * 16 + n) : 0;
   auto turn = [&](UnitShare<BITS, D>& next, int i) {
     const int t0 = 32 * walk.unit(i);
     const u32x4* unit = &stage[(i - c0) & 1][lane];
@@ -677,20 +811,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
         for (int kk = 0; kk < KK; ++kk) kop[t][kk] = unit[(t * KK + kk) * 64];
     }
     put(next, i + 1);
+    bool needed = t0 < row_end && (t0 + 32 > row_low || t0 < walk.sink_end);
+    MaskRegs<NQT> mregs;
+    if (HAS_MASK) {
+      mask_regs_from_raw<NQT>(mregs, coming, p);
+      load_mask_raw<NQT>(coming, p, mask_line, 32 * walk.unit(i + 1), g);
+      needed = needed && !walk_masked_out<D, NQT>(mregs, st);
+    }
     send(next, i + 3);
-    if (t0 < row_end && (t0 + 32 > row_low || t0 < walk.sink_end)) {
-      MaskRegs<NQT> mregs;
-      if (HAS_MASK) load_mask_regs<NQT>(mregs, p, st.mask_off, t0, g);
+    if (needed) {
       const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
       f32x4 sc[NQT][2];
       u32x4 pb[NQT];
-      walk_scores<BITS, D, NQT>([&](int t, int kk) { return AHEAD ? kop[AHEAD ? t : 0][AHEAD ? kk : 0] : unit[(t * KK + kk) * 64]; }, st, sc);
+      walk_scores<BITS, D, NQT, CHUNK>([&](int t, int kk) { return AHEAD ? kop[AHEAD ? t : 0][AHEAD ? kk : 0] : unit[(t * KK + kk) * 64]; }, st, sc);
       if constexpr (AHEAD) {
 #pragma unroll
         for (int j = 0; j < MT; ++j) vop[j] = unit[(MT + j) * 64];
       }
       walk_weights<BITS, D, NQT, HAS_MASK>(sc, st, pb, full, t0, start, walk.sink_end, g, mregs);
-      walk_output<BITS, D, NQT>([&](int j) { return AHEAD ? vop[AHEAD ? j : 0] : unit[(MT + j) * 64]; }, st, pb);
+      walk_output<BITS, D, NQT, CHUNK>([&](int j) { return AHEAD ? vop[AHEAD ? j : 0] : unit[(MT + j) * 64]; }, st, pb);
     }
     __syncthreads();
   };
@@ -705,6 +844,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
     }
     const int c1 = min(c0 + 64, i_end);
     put(even, c0);
+    if (HAS_MASK) load_mask_raw<NQT>(coming, p, mask_line, 32 * walk.unit(c0), g);
     send(even, c0 + 2);
     __syncthreads();
     int i = c0;
@@ -717,45 +857,57 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
   walk_finish<D, NQT, HAS_MASK>(st);
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt)
-    if (w_first + qt * 16 + n < R) walk_store(p, st, qt, b, part, g);
+    if (w_first + qt * 16 + n < R) walk_store(p, st, qt, b, kvh, slot, w_first + qt * 16 + n - r_first, g);
+  } while (p.shares > 0 && turns.left > 0 && turns.j < n_groups);
 }
 
-// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partitions of a query row.  A wave takes eight partitions at a time, a
-// lane the dims 2 lane, 2 lane + 1 (+ 128); WPR waves share a row (partitions in turn, joined through LDS).  The launch is a
-// chain of memory round trips, so the first eight partials are fetched before the sequence's length says how many there
-// are: the workspace holds max_parts of every row, and what is not a partial is not used.
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partial results of a query row.  A wave takes eight at a time, a lane the
+// dims 2 lane, 2 lane + 1 (+ 128); WPR waves share a row (partial results in turn, joined through LDS).  Rows of groups that
+// one workgroup covered are finished already; rows that read nothing belong to no workgroup and become 0 here.
 template <int D, int WPR>
-__global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int32_t rows_per_group, int32_t total_rows) {
+__global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int32_t total_rows) {
   constexpr int PASSES = (D + 127) / 128;
   __shared__ float join[WPR > 1 ? WPR : 1][2 * PASSES + 2][WPR > 1 ? 64 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave % WPR;
   const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;  // (b, hq, s)
   if (row >= total_rows) return;  // (WPR == 1 only: whole waves; else the grid is exact)
   const int S = p.q_len, s = (int)(row % S), hq = (int)(row / S % p.num_q_heads), b = (int)(row / S / p.num_q_heads);
-  const float* ml = p.part_ml + row * p.max_parts * 2;
-  const float* po = p.part_o + row * p.max_parts * D;
+  const int kvh = hq / p.n_rep, r = s * p.n_rep + hq % p.n_rep, qg = r / p.group_rows;
+  const int j = b * p.n_qgroups + p.n_qgroups - 1 - qg;
+  int units, share, at;  // of the row's group: units, and where they begin in the run of all units
+  if (p.part_units > 0 && p.batch * p.n_qgroups == 1) {
+    units = group_units(p, 0), share = p.part_units, at = 0;
+  } else {
+    int before = 0, total = 0;
+#pragma unroll 4
+    for (int i = lane; i < p.batch * p.n_qgroups; i += 64) {
+      const int u = group_units(p, i);
+      total += u, before += i < j ? u : 0;
+    }
+    total = wave_sum(total), at = wave_sum(before);
+    share = walk_share(p, total);
+    units = group_units(p, j);
+  }
+  const int w0 = at / share, n_parts = units > 0 ? min((at + units - 1) / share, p.shares - 1) - w0 + 1 : 0;
+  if (n_parts == 1) return;  // uniform over the row's waves
+  // workgroup w0 + i's piece lies in its first slot, except the first one's if that workgroup began with other groups
+  const int late = at % share != 0 ? 1 : 0;
+  auto place = [&](int i) { return ((int64_t)(2 * (w0 + i) + (i == 0 ? late : 0)) * p.num_kv_heads + kvh) * p.max_parts + (r - qg * p.group_rows); };
   const int d0 = 2 * lane;
   float acc[PASSES][2], M = kNegInf, L = 0.f;
 #pragma unroll
   for (int e = 0; e < PASSES; ++e) acc[e][0] = acc[e][1] = 0.f;
-  int n_parts = p.max_parts;
   for (int base = 8 * slice; base < n_parts; base += 8 * WPR) {
-    const int mine = min(base + (lane & 7), p.max_parts - 1);
-    const u32x2 pair = *reinterpret_cast<const u32x2*>(ml + 2 * mine);
+    const u32x2 pair = *reinterpret_cast<const u32x2*>(p.part_ml + 2 * place(min(base + (lane & 7), n_parts - 1)));
     u32x2 v[8][PASSES];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int e = 0; e < PASSES; ++e) {
-        v[j][e] = u32x2{0u, 0u};
-        if (base + j < p.max_parts && d0 + 128 * e < D) v[j][e] = *reinterpret_cast<const u32x2*>(po + (int64_t)(base + j) * D + d0 + 128 * e);
+        v[i][e] = u32x2{0u, 0u};
+        if (base + i < n_parts && d0 + 128 * e < D) v[i][e] = *reinterpret_cast<const u32x2*>(p.part_o + place(base + i) * D + d0 + 128 * e);
       }
-    if (base == 8 * slice) {
-      const int len = walk_len(p, b), start = walk_start(p, b, len);
-      const int r = s * p.n_rep + hq % p.n_rep, r_first = r / rows_per_group * rows_per_group;
-      n_parts = walk_parts(p, walk_of(p, len, start, r_first / p.n_rep, (min(S * p.n_rep, r_first + rows_per_group) - 1) / p.n_rep).total);
-    }
-    float m_mine = base + (lane & 7) < n_parts ? __uint_as_float(pair[0]) : kNegInf;
+    const float m_mine = base + (lane & 7) < n_parts ? __uint_as_float(pair[0]) : kNegInf;
     float top = m_mine;
     top = fmaxf(top, __shfl_xor(top, 1, 64)), top = fmaxf(top, __shfl_xor(top, 2, 64)), top = fmaxf(top, __shfl_xor(top, 4, 64));
     const float M_new = fmaxf(M, top), m_use = M_new == kNegInf ? 0.f : M_new, old = __builtin_amdgcn_exp2f(M - m_use);
@@ -764,12 +916,12 @@ __global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int
 #pragma unroll
     for (int e = 0; e < PASSES; ++e) acc[e][0] *= old, acc[e][1] *= old;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (base + j < n_parts) {  // wave-uniform
-        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_mine), j));
-        L += w * __uint_as_float(__builtin_amdgcn_readlane(pair[1], j));
+    for (int i = 0; i < 8; ++i) {
+      if (base + i < n_parts) {  // wave-uniform
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_mine), i));
+        L += w * __uint_as_float(__builtin_amdgcn_readlane(pair[1], i));
 #pragma unroll
-        for (int e = 0; e < PASSES; ++e) acc[e][0] += w * __uint_as_float(v[j][e][0]), acc[e][1] += w * __uint_as_float(v[j][e][1]);
+        for (int e = 0; e < PASSES; ++e) acc[e][0] += w * __uint_as_float(v[i][e][0]), acc[e][1] += w * __uint_as_float(v[i][e][1]);
       }
     }
   }
@@ -804,8 +956,9 @@ __global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int
 // ---- host -------------------------------------------------------------------------------------------------------
 struct WalkShape {
   int nqt;         // 0: walk_attn_kernel; else row tiles per wave of walk_rows_kernel
-  int group_rows;  // query rows per workgroup
-  int n_qgroups, part_units, max_parts;
+  int group_rows;  // query rows per group
+  int n_qgroups, shares, min_share, part_units;  // see WalkParams
+  int slot_rows;   // rows of a partial result
   size_t bytes;    // of partial results
 };
 
@@ -813,41 +966,54 @@ constexpr int walk_waves(int head_dim) { return head_dim == 256 ? 2 : 4; }  // o
 constexpr int walk_occ(int head_dim) { return head_dim == 256 ? 1 : 2; }
 constexpr int rows_occ(int head_dim, int nqt) { return head_dim == 256 || nqt > 1 ? 2 : 3; }
 
-// workspace_bytes: what partial results may take (the context is cut over no more workgroups than fit).
+// workspace_bytes: what partial results may take (the units are shared out over no more workgroups than fit).
 static WalkShape walk_shape(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, size_t workspace_bytes) {
-  WalkShape s;
+  WalkShape s = {};
   const int64_t rows = a->q_len * (int64_t)(a->num_q_heads / pool->num_kv_heads);
-  const int D = pool->head_dim;
+  const int D = pool->head_dim, heads = pool->num_kv_heads;
   s.nqt = rows <= 16 ? 0 : (rows <= 64 || D == 256 ? 1 : 2);
   s.group_rows = s.nqt == 0 ? 16 : 64 * s.nqt;
   s.n_qgroups = (int)((rows + s.group_rows - 1) / s.group_rows);
-  int64_t units = ((int64_t)a->max_seq_len + 31) / 32;
+  s.slot_rows = (int)std::min<int64_t>(rows, s.group_rows);
+  int64_t units = ((int64_t)a->max_seq_len + 31) / 32;  // of the longest group
   if (a->window > 0) units = std::min(units, ((int64_t)a->window + a->q_len) / 32 + 2 + a->sinks / 32 + 2);
   units = std::max<int64_t>(units, 1);
-  const int64_t at_once = s.nqt == 0 ? walk_waves(D) : 1;  // units a workgroup works on side by side
-  const int64_t groups = (int64_t)a->batch * pool->num_kv_heads * s.n_qgroups, cus = compute_units();
-  int64_t per = a->partition_tokens / 32, parts;
-  if (per == 0) {
-    // How many workgroups share a sequence.  One per compute unit is enough for walk_attn_kernel, whose waves fetch ahead; the
-    // others want as many as fit side by side, and twice that with few rows, where lengths may differ (a batch of drafts)
-    // and partial results are small.  A cut costs a second launch and a trip of the partial results: no share below
-    // min_share units for that.  Lengths are not known here, so a sequence that could be far longer than the others is cut
-    // at about 4096 tokens.
-    const int64_t want = s.nqt == 0 ? cus : cus * rows_occ(D, s.nqt) * (s.nqt == 1 && rows <= 64 ? 2 : 1);
-    const int64_t min_share = s.nqt == 0 ? 4 : 12;
-    parts = std::max<int64_t>((units + 64) / 128, groups >= want ? 1 : (want + groups - 1) / groups);
-    parts = std::max<int64_t>(std::min(parts, units / min_share), 1);
-    per = (units + parts - 1) / parts;
+  s.min_share = s.nqt == 0 ? walk_waves(D) : 1;  // units a workgroup works on side by side
+  const int64_t n_groups = (int64_t)a->batch * s.n_qgroups, groups = n_groups * heads;
+  // Workgroups that run side by side.  One per compute unit is enough for walk_attn_kernel, whose waves fetch ahead.
+  const int64_t slots = (int64_t)compute_units() * (s.nqt == 0 ? 1 : rows_occ(D, s.nqt));
+  int64_t shares = 0;
+  if (a->partition_tokens > 0) {
+    s.part_units = (a->partition_tokens / 32 + s.min_share - 1) / s.min_share * s.min_share;
+    shares = n_groups == 1 ? (units + s.part_units - 1) / s.part_units : (n_groups * units + s.part_units - 1) / s.part_units;
+    if (units <= s.part_units && n_groups == 1) shares = 0;
+  } else {
+    // Sharing costs a second launch and a trip of the partial results, some 5 us: not for groups of few units.  It pays where a
+    // workgroup per group would leave much of the GPU idle -- in its last round, or because some sequence may be far
+    // longer than the others (lengths are not known here, only their bound).
+    const double idle = (double)((groups + slots - 1) / slots * slots) / (double)groups;
+    const int64_t few = s.nqt == 0 ? 8 : 16;
+    if (units > few && (units > 160 || idle > 1.2)) {
+      shares = std::max<int64_t>(slots / heads, 1);
+      if (s.nqt != 0) s.min_share = 4;
+      if (n_groups == 1) {
+        s.part_units = (int)std::max<int64_t>((units + shares - 1) / shares, s.nqt == 0 ? 4 : 12);
+        s.part_units = (s.part_units + s.min_share - 1) / s.min_share * s.min_share;
+        shares = (units + s.part_units - 1) / s.part_units;
+        if (shares == 1) shares = 0;
+      }
+    }
   }
-  per = (std::max<int64_t>(per, 1) + at_once - 1) / at_once * at_once;
-  parts = (units + per - 1) / per;
-  const size_t one = (size_t)a->batch * a->num_q_heads * a->q_len * (D + 2) * sizeof(float);
-  if (parts > 1 && workspace_bytes / one < (size_t)parts) {
-    parts = std::max<int64_t>((int64_t)(workspace_bytes / one), 1);
-    per = (units + parts - 1) / parts;
+  const size_t one = (size_t)heads * 2 * s.slot_rows * (D + 2) * sizeof(float);  // of a workgroup per KV head
+  if (shares > 0 && workspace_bytes / one < (size_t)shares) {
+    shares = (int64_t)(workspace_bytes / one);
+    if (shares <= n_groups) shares = 0;  // (a workgroup per group does as well)
+    s.part_units = 0;
+    if (shares > 0 && n_groups == 1) s.part_units = (int)(((units + shares - 1) / shares + s.min_share - 1) / s.min_share * s.min_share);
   }
-  s.part_units = (int)per, s.max_parts = (int)parts;
-  s.bytes = parts > 1 ? one * (size_t)parts : 0;
+  s.shares = (int)shares;
+  if (shares == 0) s.part_units = 0;
+  s.bytes = one * (size_t)shares;
   return s;
 }
 
@@ -891,14 +1057,15 @@ int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, con
   p.causal = a->causal;
   p.scale = a->scale, p.scale_log2 = a->scale * kLog2e;
   p.window = std::min(a->window, 1 << 30), p.sinks = std::min(a->sinks, 1 << 30);  // (sums with them stay below 2^31)
-  p.n_qgroups = sh.n_qgroups, p.part_units = sh.part_units, p.max_parts = sh.max_parts;
+  p.n_qgroups = sh.n_qgroups, p.group_rows = sh.group_rows, p.max_parts = sh.slot_rows;
+  p.shares = sh.shares, p.min_share = sh.min_share, p.part_units = sh.part_units;
   const size_t rows = (size_t)a->batch * a->num_q_heads * a->q_len;
   PACE_REQUIRE(rows < ((size_t)1 << 31), "%s: too many query rows", who);
-  if (sh.max_parts > 1) {
+  if (sh.shares > 0) {
     p.part_o = static_cast<float*>(a->workspace);
-    p.part_ml = p.part_o + rows * sh.max_parts * pool->head_dim;
+    p.part_ml = p.part_o + (size_t)sh.shares * 2 * pool->num_kv_heads * sh.slot_rows * pool->head_dim;
   }
-  p.total_items = (long long)a->batch * sh.max_parts * pool->num_kv_heads * sh.n_qgroups;
+  p.total_items = (sh.shares > 0 ? (long long)sh.shares : (long long)a->batch * sh.n_qgroups) * pool->num_kv_heads;
   PACE_REQUIRE(p.total_items < (1ll << 31), "%s: grid too large", who);
   if (a->k_new)  // the new tokens first: they are read back from the pool like all others
     if (int rc = pace_kv_append_paged_at(pool, a->k_new, a->v_new, a->new_stride_b, a->new_stride_h, a->new_stride_t, a->batch, a->n_new,
@@ -912,10 +1079,11 @@ int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, con
     } else {
       if (masked) launch_walk_kernel<16, D, true>(p, sh.nqt, stream); else launch_walk_kernel<16, D, false>(p, sh.nqt, stream);
     }
-    if (sh.max_parts > 8)
-      hipLaunchKernelGGL((walk_merge_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, p, sh.group_rows, (int32_t)rows);
-    else if (sh.max_parts > 1)
-      hipLaunchKernelGGL((walk_merge_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p, sh.group_rows, (int32_t)rows);
+    // few groups, many workgroups each: four waves to a row
+    if (sh.shares > 4 * (int64_t)a->batch * sh.n_qgroups)
+      hipLaunchKernelGGL((walk_merge_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, p, (int32_t)rows);
+    else if (sh.shares > 0)
+      hipLaunchKernelGGL((walk_merge_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p, (int32_t)rows);
   });
   PACE_HIP_CHECK(hipGetLastError());
   return PACE_KV_OK;
