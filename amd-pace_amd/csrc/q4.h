@@ -82,49 +82,89 @@ __device__ __forceinline__ uint32_t q4_or_bits() {
   return b;
 }
 
-// Quantises a group of 32 values held by four neighbouring lanes (eight each, lanes 4 k .. 4 k + 3): this lane's codes as
-// a dword, and the group's step and middle.  All four lanes have to be active together.
+// Quantises a group of 32 bf16 values held by four neighbouring lanes (eight each, lanes 4 k .. 4 k + 3, all active): the group's
+// step and middle, and this lane's codes (+ 8) as byte 2 of eight words.
 //
-// Codes are decided as by exact arithmetic: in single precision (x - m) * (1 / s) is off by less than 2^-18 of a step
-// for every quotient that is not cut to -8 or 7 anyway, so only a quotient within 2^-16 of a border (a few values in
-// 100 000) is divided again in double precision.
-__device__ __forceinline__ uint32_t q4_quantise(const float (&x_in)[8], _Float16& s_out, _Float16& m_out) {
-  float x[8], lo = kQ4Clamp, hi = -kQ4Clamp;
+// Codes are decided as by exact arithmetic.  y = x / s + (136 - m / s), one multiply-add with the reciprocal, lies in [128, 144): its
+// last place is 2^-16, and as |m / s| <= 64 (else the group takes the other way) it is off by less than one: 2^-17 each for
+// the added constant and for the sum, 9 * 2^-23 for the reciprocal.  Adding one half to the bits rounds it, the code is
+// then byte 2, and a fraction within two places of a border (6 values in 100 000) is decided again.
+// a - b == d + q4_rest(a, b, d) exactly, d the rounded difference.
+__device__ __forceinline__ float q4_rest(float a, float b, float d) {
+  const float back = d - a;
+  return (a - (d - back)) - (b + back);
+}
+template <int PERM>  // the value of another of the four lanes
+__device__ __forceinline__ float q4_quad(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), PERM, 0xf, 0xf, true));
+}
+__device__ __forceinline__ void bf16x8_to_f32(u32x4 raw, float (&x)[8]);
+__device__ __forceinline__ void q4_quantise(u32x4 raw, uint32_t (&q)[8], _Float16& s_out, _Float16& m_out) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  float x[8];
+  bf16x8_to_f32(raw, x);
+  // magnitudes above 2^15 and NaN are rare: looked for on the bit patterns (0x4700 is 2^15), held only where there are any
+  u16x2 top = {0, 0};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    x[e] = x_in[e] == x_in[e] ? fminf(fmaxf(x_in[e], -kQ4Clamp), kQ4Clamp) : 0.f;
-    lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
+  for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, raw[e] & 0x7fff7fffu));
+  if (top[0] > 0x4700 || top[1] > 0x4700) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] == x[e] ? fminf(fmaxf(x[e], -kQ4Clamp), kQ4Clamp) : 0.f;
   }
-  lo = fminf(lo, __shfl_xor(lo, 1, 64)), hi = fmaxf(hi, __shfl_xor(hi, 1, 64));
-  lo = fminf(lo, __shfl_xor(lo, 2, 64)), hi = fmaxf(hi, __shfl_xor(hi, 2, 64));
-  // the least half with 15 s >= hi - lo: the nearest half to the quotient, then one step up or down (halves >= 0 are in
-  // the order of their bit patterns; 15 s and the width are exact in double precision)
-  const double width = (double)hi - (double)lo;
-  uint32_t sb = half_bits((_Float16)((hi - lo) * (1.f / 15.f)));
-  if (15.0 * (double)(float)half_from(sb) < width) ++sb;
-  else if (sb > 0 && 15.0 * (double)(float)half_from(sb - 1) >= width) --sb;
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) lo = __builtin_elementwise_minimum(lo, x[e]), hi = __builtin_elementwise_maximum(hi, x[e]);
+  lo = __builtin_elementwise_minimum(lo, q4_quad<0xb1>(lo)), hi = __builtin_elementwise_maximum(hi, q4_quad<0xb1>(hi));
+  lo = __builtin_elementwise_minimum(lo, q4_quad<0x4e>(lo)), hi = __builtin_elementwise_maximum(hi, q4_quad<0x4e>(hi));
+  // The least half with 15 s >= hi - lo: the nearest half to the quotient, then one step up or down (halves >= 0 are in the order of
+  // their bit patterns).  The width is kept as the sum of the rounded difference and its error, so the comparisons are exact:
+  // 15 s - width is small only where it is a short number.
+  const float width = hi - lo, rest = q4_rest(hi, lo, width);
+  uint32_t sb = half_bits((_Float16)(width * (1.f / 15.f)));
+  if (__builtin_fmaf(15.f, (float)half_from(sb), -width) < rest) ++sb;
+  else if (sb > 0 && __builtin_fmaf(15.f, (float)half_from(sb - 1), -width) >= rest) --sb;
   const _Float16 s = half_from(sb);
   const float sf = (float)s;
   const _Float16 m = (_Float16)__builtin_fmaf(8.f, sf, lo);
   const float mf = (float)m;
-  const float inv = sf > 0.f ? 1.f / sf : 0.f;
-  float q[8];
-  bool border = false;
+  const float inv = sf > 0.f ? __builtin_amdgcn_rcpf(sf) : 0.f;
+  const float add = __builtin_fmaf(-mf, inv, 136.f);
+  u16x2 frac = {0xffff, 0xffff};  // how far above a border the values are
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float t = (x[e] - mf) * inv;
-    q[e] = __builtin_rintf(t);
-    border = border || fabsf(t - q[e]) > 0.5f - 0x1p-16f;
-  }
-  if (border && sf > 0.f) {
+  for (int e = 0; e < 8; ++e) q[e] = __float_as_uint(__builtin_amdgcn_fmed3f(__builtin_fmaf(x[e], inv, add), 128.f, 143.f)) + 0x8002u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = (float)__builtin_rint(((double)x[e] - (double)mf) / (double)sf);
+  for (int i = 0; i < 4; ++i) frac = __builtin_elementwise_min(frac, __builtin_bit_cast(u16x2, __builtin_amdgcn_perm(q[2 * i + 1], q[2 * i], 0x05040100u)));
+  if ((frac[0] < 4 || frac[1] < 4 || fabsf(add - 136.f) > 64.f) && sf > 0.f) {
+    // Exactly: x - m as a rounded difference and its error (q4_rest), against the border (f + 1/2) s, a number of 16 bits.  The
+    // difference of the two is exact where it is small, so its sign is right everywhere.
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = x[e] - mf, f = floorf(fminf(fmaxf(d * inv, -16.f), 16.f));
+      float rest = q4_rest(x[e], mf, d);
+      if (fabsf(rest) <= 0x1p-54f * fabsf(d)) rest = 0.f;  // (not seen in double precision, in which the format is defined)
+      const float over = __builtin_fmaf(-(f + 0.5f), sf, d) + rest;
+      const int code = (int)f + (over > 0.f || (over == 0.f && ((int)f & 1)) ? 1 : 0);
+      q[e] = (uint32_t)(8 + min(max(code, -8), 7)) << 16;
+    }
   }
+  s_out = s, m_out = m;
+}
+
+// The eight codes in a dword's bits (see above), and as eight bytes.
+__device__ __forceinline__ uint32_t q4_pack(const uint32_t (&q)[8]) {
   uint32_t w = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w |= (uint32_t)((int)fminf(fmaxf(q[e], -8.f), 7.f) + 8) << q4_bit(e);
-  s_out = s, m_out = m;
+  for (int i = 0; i < 4; ++i) w |= __builtin_amdgcn_perm(q[2 * i + 1], q[2 * i], 0x0c060c02u) << (4 * i);
   return w;
+}
+__device__ __forceinline__ u32x2 q4_bytes(const uint32_t (&q)[8]) {
+  u32x2 r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t lo = __builtin_amdgcn_perm(q[4 * h + 1], q[4 * h], 0x0c0c0602u), hi = __builtin_amdgcn_perm(q[4 * h + 3], q[4 * h + 2], 0x06020c0cu);
+    r[h] = lo | hi;
+  }
+  return r;
 }
 
 __device__ __forceinline__ void bf16x8_to_f32(u32x4 raw, float (&x)[8]) {

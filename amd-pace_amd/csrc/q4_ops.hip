@@ -6,118 +6,145 @@
 namespace pace_kv {
 
 // ---------------------------------------------------------------------------------
-// Append.  One workgroup of 2 D threads takes up to 16 tokens of one (sequence, KV head): thread (token, chunk) reads eight
+// Append.  A workgroup of 2 D threads takes up to 16 tokens of one (sequence, KV head) at a time: thread (token, chunk) has eight
 // dims of K and of V (16 bytes each), four neighbouring threads make a group of 32 and agree on its step and middle in
 // registers.  K codes are a token's own dword and are stored from where they are made; a V code dword holds eight
 // tokens of one dim, so the codes meet in LDS, one byte each, and every thread puts one dword together.
-//   PAGED: the tokens of one destination block.  A V dword has one writer, the block's workgroup: where the append
-//   covers only some of its eight tokens the dword is read, changed and written back.
-//   by slot: 16 consecutive tokens of the input, wherever their slots lie.  Tokens of one V dword may then sit in two
-//   workgroups; a dword not covered in full is changed by atomics on its own bits (each bit has one writer as long as
-//   no slot is named twice, so the order does not matter).
 // ---------------------------------------------------------------------------------
-template <int D, bool PAGED>
-__global__ __launch_bounds__(2 * D) void q4_append_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
-                                                          const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh, int64_t st,
-                                                          int32_t n_tokens, int32_t groups_x, const AppendDest dest) {
+// Quantises one token's eight dims (chunk c) of K and V: K and the scales into the slabs, V codes as bytes to `bytes`.  The threads of
+// a token come here together.
+template <int D>
+__device__ __forceinline__ void q4_store_token(uint8_t* kslab, uint8_t* vslab, int tok, int c, u32x4 kraw, u32x4 vraw, uint8_t* bytes) {
   using L = Q4<D>;
+  const int kk = c / 4, g = c % 4;
+  uint32_t q[8];
+  _Float16 s, m;
+  q4_quantise(kraw, q, s, m);
+  uint32_t* k32 = reinterpret_cast<uint32_t*>(kslab);
+  k32[L::k_code(q4_tile(tok), g, q4_slot(tok), kk)] = q4_pack(q);
+  if (g == 0) k32[L::k_scale(q4_tile(tok), q4_slot(tok), kk)] = half_bits(s) | (half_bits(m) << 16);
+  q4_quantise(vraw, q, s, m);
+  if (g == 0) {
+    uint16_t* v16 = reinterpret_cast<uint16_t*>(vslab);
+    v16[L::v_scale(kk, tok)] = (uint16_t)half_bits(s);
+    v16[L::v_scale(kk, tok) + 16 * L::G] = (uint16_t)half_bits(m);
+  }
+  *reinterpret_cast<u32x2*>(bytes) = q4_bytes(q);
+}
+// The dim of V dword r of a token half, in slab order: a wave's dwords are contiguous.
+template <int D>
+__device__ __forceinline__ int q4_v_dim(int r) {
+  constexpr int VC = Q4<D>::VC;
+  return 16 * (r / (16 * VC) * VC + r % VC) + r / VC % 16;
+}
+
+// By position: one destination block of one (sequence, KV head).  A V dword has one writer, its block's workgroup: where the append
+// covers only some of its eight tokens it is read, changed and written back.
+// 8 prompts of 4096 tokens, 8 heads of 128: 48 us for 176 MB, 41 us with the quantising left out.  Several blocks per workgroup with
+// the next one's rows under way measured 3 .. 8 us more: eight workgroups per compute unit hide the loads already.
+template <int D>
+__global__ __launch_bounds__(2 * D) void q4_append_paged_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
+                                                                const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh, int64_t st,
+                                                                int32_t n_tokens, int32_t groups_x, const AppendDest dest) {
   constexpr int CHUNKS = D / 8, BT = PACE_KV_BLOCK_TOKENS, ROW = D + 8;
   __shared__ __attribute__((aligned(8))) uint8_t codes[BT * ROW];  // V codes, token-major
-  __shared__ int64_t slot_of[BT];                                  // by slot: the tokens' slots (-1: none)
-  const int H = pool.num_kv_heads;
-  const int x = (int)(blockIdx.x % (uint32_t)groups_x), h = (int)(blockIdx.x / (uint32_t)groups_x % (uint32_t)H);
-  const int64_t b = blockIdx.x / (uint32_t)groups_x / (uint32_t)H;
+  const uint32_t H = (uint32_t)pool.num_kv_heads;
+  const int x = (int)(blockIdx.x % (uint32_t)groups_x), h = (int)(blockIdx.x / (uint32_t)groups_x % H);
+  const int64_t b = blockIdx.x / (uint32_t)groups_x / H;
   const int i = threadIdx.x / CHUNKS, c = threadIdx.x % CHUNKS;  // this thread's token (of 16) and eight dims
-  int64_t t;      // token of the input
-  int64_t blk;    // destination block
-  int off;        // token slot in it
-  int first = 0, count = 0;  // PAGED: block tokens first .. first + count - 1 are written
-  bool live;
-  if (PAGED) {
-    const int64_t pos0 = (int64_t)dest.seq_lens[b] + dest.pos_offset + (dest.offset_dev ? *dest.offset_dev : 0);
-    const int64_t jb = (pos0 > 0 ? pos0 : 0) / BT + x;
-    if (jb >= dest.table_stride) return;  // uniform over the workgroup, like the next two
-    const int64_t lo = max(pos0, jb * BT), hi = min(pos0 + n_tokens, jb * BT + BT);
-    if (lo >= hi) return;
-    blk = dest.table[b * dest.table_stride + jb];
-    if (blk < 0 || blk >= pool.num_blocks) return;  // never write outside the pool
-    first = (int)(lo - jb * BT), count = (int)(hi - lo);
-    off = i;
-    t = jb * BT + i - pos0;
-    live = i >= first && i < first + count;
-  } else {
-    t = (int64_t)x * BT + i;
-    int64_t slot = t < n_tokens ? dest.slots[b * n_tokens + t] : -1;
-    if (slot < 0 || slot / BT >= pool.num_blocks) slot = -1;
-    if (c == 0) slot_of[i] = slot;
-    live = slot >= 0;
-    blk = live ? slot / BT : 0;
-    off = live ? (int)(slot % BT) : 0;
+  const int64_t pos0 = (int64_t)dest.seq_lens[b] + dest.pos_offset + (dest.offset_dev ? *dest.offset_dev : 0);
+  const int64_t jb = (pos0 > 0 ? pos0 : 0) / BT + x;
+  if (jb >= dest.table_stride) return;  // uniform over the workgroup, like the next two
+  const int64_t lo = max(pos0, jb * BT), hi = min(pos0 + n_tokens, jb * BT + BT);
+  if (lo >= hi) return;
+  const int64_t blk = dest.table[b * dest.table_stride + jb];
+  const int first = (int)(lo - jb * BT), past = (int)(hi - jb * BT);
+  const bool live = i >= first && i < past;
+  // The rows are asked for next to the block id, not behind it.
+  u32x4 kraw = {0u, 0u, 0u, 0u}, vraw = {0u, 0u, 0u, 0u};
+  if (live) {
+    const int64_t src = b * sb + (int64_t)h * sh + (jb * BT + i - pos0) * st + c * 8;
+    kraw = load16_stream(k_new + src), vraw = load16_stream(v_new + src);
   }
+  if (blk < 0 || blk >= pool.num_blocks) return;  // never write outside the pool
   uint8_t* kslab = static_cast<uint8_t*>(pool.k) + blk * pool.k_block_stride + (int64_t)h * pool.k_head_stride;
   uint8_t* vslab = static_cast<uint8_t*>(pool.v) + blk * pool.v_block_stride + (int64_t)h * pool.v_head_stride;
-  const int kk = c / 4, g = c % 4;
-  if (live) {  // the same for a token's threads, so for every group of four
+  uint32_t* const at = reinterpret_cast<uint32_t*>(vslab) + threadIdx.x;  // this thread's V dword: (token half, dim)
+  const int half = threadIdx.x / D, dim = q4_v_dim<D>(threadIdx.x % D);
+  uint32_t lower = 0, upper = 0;  // which of its bits are written: the same for the whole workgroup
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    lower |= e >= first && e < past ? 15u << q4_bit(e) : 0u;
+    upper |= 8 + e >= first && 8 + e < past ? 15u << q4_bit(e) : 0u;
+  }
+  const uint32_t mask = half ? upper : lower;
+  uint32_t old = 0;
+  if (mask != 0u && mask != 0xffffffffu) old = *at;
+  if (live) q4_store_token<D>(kslab, vslab, i, c, kraw, vraw, &codes[i * ROW + c * 8]);
+  __syncthreads();
+  uint32_t w = 0;
+  if (mask == 0xffffffffu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= (uint32_t)codes[(8 * half + e) * ROW + dim] << q4_bit(e);
+    *at = w;
+  } else if (mask != 0u) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= (codes[(8 * half + e) * ROW + dim] & 15u) << q4_bit(e);  // (tokens not written: anything)
+    *at = (old & ~mask) | (w & mask);
+  }
+}
+
+// By slot: 16 consecutive tokens of the input, wherever their slots lie.  Tokens of one V dword may then sit in two workgroups; a
+// dword not covered in full is changed by atomics on its own bits (each bit has one writer as long as no slot is named
+// twice, so the order does not matter).
+template <int D>
+__global__ __launch_bounds__(2 * D) void q4_append_slots_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
+                                                                const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh, int64_t st,
+                                                                int32_t n_tokens, int32_t groups_x, const AppendDest dest) {
+  constexpr int CHUNKS = D / 8, BT = PACE_KV_BLOCK_TOKENS, ROW = D + 8;
+  __shared__ __attribute__((aligned(8))) uint8_t codes[BT * ROW];
+  __shared__ int64_t slot_of[BT];  // the tokens' slots (-1: none)
+  const uint32_t H = (uint32_t)pool.num_kv_heads;
+  const int x = (int)(blockIdx.x % (uint32_t)groups_x), h = (int)(blockIdx.x / (uint32_t)groups_x % H);
+  const int64_t b = blockIdx.x / (uint32_t)groups_x / H;
+  const int i = threadIdx.x / CHUNKS, c = threadIdx.x % CHUNKS;
+  const int64_t t = (int64_t)x * BT + i;
+  int64_t slot = t < n_tokens ? dest.slots[b * n_tokens + t] : -1;
+  if (slot < 0 || slot / BT >= pool.num_blocks) slot = -1;
+  if (c == 0) slot_of[i] = slot;
+  if (__syncthreads_or(slot >= 0) == 0) return;
+  uint8_t* const k_head = static_cast<uint8_t*>(pool.k) + (int64_t)h * pool.k_head_stride;
+  uint8_t* const v_head = static_cast<uint8_t*>(pool.v) + (int64_t)h * pool.v_head_stride;
+  if (slot >= 0) {
     const int64_t src = b * sb + (int64_t)h * sh + t * st + c * 8;
     const u32x4 kraw = load16_stream(k_new + src), vraw = load16_stream(v_new + src);
-    float xs[8];
-    _Float16 s, m;
-    bf16x8_to_f32(kraw, xs);
-    const uint32_t kw = q4_quantise(xs, s, m);
-    uint32_t* k32 = reinterpret_cast<uint32_t*>(kslab);
-    k32[L::k_code(q4_tile(off), g, q4_slot(off), kk)] = kw;
-    if (g == 0) k32[L::k_scale(q4_tile(off), q4_slot(off), kk)] = half_bits(s) | (half_bits(m) << 16);
-    bf16x8_to_f32(vraw, xs);
-    const uint32_t vw = q4_quantise(xs, s, m);
-    if (g == 0) {
-      uint16_t* v16 = reinterpret_cast<uint16_t*>(vslab);
-      v16[L::v_scale(kk, off)] = (uint16_t)half_bits(s);
-      v16[L::v_scale(kk, off) + 16 * L::G] = (uint16_t)half_bits(m);
-    }
-    u32x2 bytes = {0u, 0u};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bytes[e >> 2] |= ((vw >> q4_bit(e)) & 15u) << (8 * (e & 3));
-    *reinterpret_cast<u32x2*>(&codes[i * ROW + c * 8]) = bytes;
+    q4_store_token<D>(k_head + slot / BT * pool.k_block_stride, v_head + slot / BT * pool.v_block_stride, (int)(slot % BT), c, kraw, vraw,
+                      &codes[i * ROW + c * 8]);
   }
   __syncthreads();
-  // This thread's V dword: (token half, dim), dims in the order of the slab, so that a wave's stores are contiguous.
-  const int o = threadIdx.x, half = o / D, r = o % D;
-  const int dim = 16 * (r / (16 * L::VC) * L::VC + r % L::VC) + r / L::VC % 16;
-  if (PAGED) {
-    uint32_t* at = reinterpret_cast<uint32_t*>(vslab) + o;
+  // Every V dword a token of this workgroup lies in, found at its first token here (uniform over the workgroup); the two thread
+  // halves take the dwords in turn.
+  const int half = threadIdx.x / D, r = threadIdx.x % D, dim = q4_v_dim<D>(r);
+  int turn = 0;
+  for (int a = 0; a < BT; ++a) {
+    const int64_t key = slot_of[a] < 0 ? -1 : slot_of[a] / 8;
+    bool seen = key < 0;
+    for (int e = 0; e < a; ++e) seen = seen || (slot_of[e] >= 0 && slot_of[e] / 8 == key);
+    if (seen) continue;
+    if ((turn++ & 1) != half) continue;
     uint32_t w = 0, mask = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int tok = 8 * half + e;
-      if (tok >= first && tok < first + count) w |= (uint32_t)codes[tok * ROW + dim] << q4_bit(e), mask |= 15u << q4_bit(e);
+    for (int e = a; e < BT; ++e) {
+      if (slot_of[e] < 0 || slot_of[e] / 8 != key) continue;
+      const int bit = q4_bit((int)(slot_of[e] % 8));
+      w = (w & ~(15u << bit)) | ((uint32_t)codes[e * ROW + dim] << bit);
+      mask |= 15u << bit;
     }
-    if (mask == 0xffffffffu) *at = w;
-    else if (mask != 0u) *at = (*at & ~mask) | w;
-  } else {
-    // Every V dword a token of this workgroup lies in, found at its first token here (uniform over the workgroup); the two
-    // thread halves take the dwords in turn.
-    int turn = 0;
-    for (int a = 0; a < BT; ++a) {
-      const int64_t key = slot_of[a] < 0 ? -1 : slot_of[a] / 8;
-      bool seen = key < 0;
-      for (int e = 0; e < a; ++e) seen = seen || (slot_of[e] >= 0 && slot_of[e] / 8 == key);
-      if (seen) continue;
-      if ((turn++ & 1) != half) continue;
-      uint32_t w = 0, mask = 0;
-      for (int e = a; e < BT; ++e) {
-        if (slot_of[e] < 0 || slot_of[e] / 8 != key) continue;
-        const int bit = q4_bit((int)(slot_of[e] % 8));
-        w = (w & ~(15u << bit)) | ((uint32_t)codes[e * ROW + dim] << bit);
-        mask |= 15u << bit;
-      }
-      uint32_t* at = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(pool.v) + key / 2 * pool.v_block_stride + (int64_t)h * pool.v_head_stride) +
-                     (key % 2) * D + r;
-      if (mask == 0xffffffffu) {
-        *at = w;
-      } else {
-        atomicAnd(at, ~mask);
-        atomicOr(at, w);
-      }
+    uint32_t* at = reinterpret_cast<uint32_t*>(v_head + key / 2 * pool.v_block_stride) + (key % 2) * D + r;
+    if (mask == 0xffffffffu) {
+      *at = w;
+    } else {
+      atomicAnd(at, ~mask);
+      atomicOr(at, w);
     }
   }
 }
@@ -127,16 +154,40 @@ __global__ __launch_bounds__(2 * D) void q4_append_kernel(pace_kv_pool_t pool, c
 // (token, chunk) makes eight dims of K from one code dword, and eight dims of V from the eight dwords its token has a
 // code in, which pass through LDS.
 // ---------------------------------------------------------------------------------
+// packed_entry() with the owner found by the lanes of a wave side by side: 64 sequences per memory round trip where the bisection
+// takes one per step.  For grids that are on the GPU all at once, whose time is a chain of such trips (5 sequences:
+// the same 4.3 us; 64: 4.9 -> 4.0 us); a long grid hides them and pays for the vector work (130 k tokens of 64
+// sequences: 134 us by bisection, 158 us this way).
+__device__ __forceinline__ void q4_packed_entry(const int32_t* __restrict__ cu, int batch, int H, unsigned entry, int lane, int& b, int& h, int& j) {
+  for (int base = 0;; base += 64) {
+    const int i = min(base + lane, batch - 1);
+    const int from = cu[i], to = cu[i + 1];
+    const uint64_t begun = __ballot(base + lane < batch && (int64_t)(from / PACE_KV_BLOCK_TOKENS + i) * H <= (int64_t)entry);
+    if (begun == ~0ull && base + 64 < batch) {
+      const int next = cu[base + 64];
+      if ((int64_t)(next / PACE_KV_BLOCK_TOKENS + base + 64) * H <= (int64_t)entry) continue;  // uniform: the same for every lane
+    }
+    const int l = 63 - __builtin_clzll(begun);  // sequence `base` has begun: bit 0 is set
+    b = base + l;
+    const int first = __builtin_amdgcn_readlane(from, l) / PACE_KV_BLOCK_TOKENS + b;
+    const int n = __builtin_amdgcn_readlane(to, l) / PACE_KV_BLOCK_TOKENS + b + 1 - first;  // >= 1
+    const int r = (int)((int64_t)entry - (int64_t)first * H);
+    h = min(r / n, H - 1), j = r % n;
+    return;
+  }
+}
+
 template <int D, bool PACKED>
 __global__ __launch_bounds__(2 * D) void q4_gather_kernel(pace_kv_pool_t pool, const int32_t* __restrict__ table, int32_t table_stride,
                                                           const int32_t* __restrict__ seq_lens, int32_t len_bias, int32_t n_rep,
-                                                          int32_t n_blocks, const GatherOut out) {
+                                                          int32_t n_blocks, int32_t side_by_side, const GatherOut out) {
   using L = Q4<D>;
   constexpr int CHUNKS = D / 8, BT = PACE_KV_BLOCK_TOKENS;
   __shared__ uint32_t vc[2 * D];
   int j, b, h;
   if (PACKED) {
-    packed_entry(out.cu_seqlens, out.batch, pool.num_kv_heads, blockIdx.x, b, h, j);
+    if (side_by_side) q4_packed_entry(out.cu_seqlens, out.batch, pool.num_kv_heads, blockIdx.x, threadIdx.x & 63, b, h, j);
+    else packed_entry(out.cu_seqlens, out.batch, pool.num_kv_heads, blockIdx.x, b, h, j);
   } else {
     j = (int)(blockIdx.x % (uint32_t)n_blocks);
     h = (int)(blockIdx.x / (uint32_t)n_blocks % (uint32_t)pool.num_kv_heads);
@@ -197,21 +248,22 @@ __global__ __launch_bounds__(2 * D) void q4_gather_kernel(pace_kv_pool_t pool, c
 int launch_q4_append(const char* who, const pace_kv_pool_t* pool, const void* k_new, const void* v_new, int64_t stride_b,
                      int64_t stride_h, int64_t stride_t, int32_t batch, int32_t n_tokens, const AppendDest& dest, bool paged,
                      hipStream_t stream) {
-  // PAGED: the most blocks n_tokens consecutive positions can touch; by slot: runs of 16 input tokens
-  const int64_t groups = paged ? ((int64_t)n_tokens + PACE_KV_BLOCK_TOKENS - 2) / PACE_KV_BLOCK_TOKENS + 1
-                               : ((int64_t)n_tokens + PACE_KV_BLOCK_TOKENS - 1) / PACE_KV_BLOCK_TOKENS;
-  const int64_t grid = groups * pool->num_kv_heads * batch;
-  PACE_REQUIRE(grid < (int64_t)1 << 31, "%s: grid too large", who);
   const uint16_t* k = static_cast<const uint16_t*>(k_new);
   const uint16_t* v = static_cast<const uint16_t*>(v_new);
+  const int64_t rows = (int64_t)pool->num_kv_heads * batch;
+  // the most blocks n_tokens consecutive positions can touch; by slot: runs of 16 input tokens
+  const int64_t blocks = paged ? ((int64_t)n_tokens + PACE_KV_BLOCK_TOKENS - 2) / PACE_KV_BLOCK_TOKENS + 1
+                               : ((int64_t)n_tokens + PACE_KV_BLOCK_TOKENS - 1) / PACE_KV_BLOCK_TOKENS;
+  const int64_t grid = blocks * rows;
+  PACE_REQUIRE(grid < (int64_t)1 << 31, "%s: grid too large", who);
   for_head_dim(pool->head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (paged)
-      hipLaunchKernelGGL((q4_append_kernel<D, true>), dim3((unsigned)grid), dim3(2 * D), 0, stream, *pool, k, v, stride_b, stride_h, stride_t,
-                         n_tokens, (int32_t)groups, dest);
+      hipLaunchKernelGGL((q4_append_paged_kernel<D>), dim3((unsigned)grid), dim3(2 * D), 0, stream, *pool, k, v, stride_b, stride_h, stride_t,
+                         n_tokens, (int32_t)blocks, dest);
     else
-      hipLaunchKernelGGL((q4_append_kernel<D, false>), dim3((unsigned)grid), dim3(2 * D), 0, stream, *pool, k, v, stride_b, stride_h, stride_t,
-                         n_tokens, (int32_t)groups, dest);
+      hipLaunchKernelGGL((q4_append_slots_kernel<D>), dim3((unsigned)grid), dim3(2 * D), 0, stream, *pool, k, v, stride_b, stride_h, stride_t,
+                         n_tokens, (int32_t)blocks, dest);
   });
   PACE_HIP_CHECK(hipGetLastError());
   return PACE_KV_OK;
@@ -223,14 +275,15 @@ int launch_q4_gather(const char* who, const pace_kv_pool_t* pool, const int32_t*
   const int64_t grid = packed ? ((int64_t)out.total_rows / PACE_KV_BLOCK_TOKENS + batch) * pool->num_kv_heads
                               : n_blocks * pool->num_kv_heads * batch;
   PACE_REQUIRE(grid < (int64_t)1 << 31, "%s: grid too large", who);
+  const int32_t side_by_side = grid <= 8 * (int64_t)compute_units() ? 1 : 0;
   for_head_dim(pool->head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (packed)
       hipLaunchKernelGGL((q4_gather_kernel<D, true>), dim3((unsigned)grid), dim3(2 * D), 0, stream, *pool, block_table, table_stride, seq_lens,
-                         seq_len_bias, n_rep, (int32_t)n_blocks, out);
+                         seq_len_bias, n_rep, (int32_t)n_blocks, side_by_side, out);
     else
       hipLaunchKernelGGL((q4_gather_kernel<D, false>), dim3((unsigned)grid), dim3(2 * D), 0, stream, *pool, block_table, table_stride, seq_lens,
-                         seq_len_bias, n_rep, (int32_t)n_blocks, out);
+                         seq_len_bias, n_rep, (int32_t)n_blocks, side_by_side, out);
   });
   PACE_HIP_CHECK(hipGetLastError());
   return PACE_KV_OK;
