@@ -1284,10 +1284,11 @@ extern "C" size_t pace_paged_attn_workspace_for(const pace_kv_pool_t* pool, cons
     return 0;
   if (pool_is_q4(pool) || args->window > 0) return walk_workspace_bytes(pool, args);
   if (pool_is_f32(pool)) {
-    // (what helps a batch that leaves compute units idle: up to 64 workgroups per sequence)
+    // (what helps a batch that leaves compute units idle: up to 64 workgroups per sequence, 64 MiB at most)
     const int64_t rows = (int64_t)args->q_len * (args->num_q_heads / pool->num_kv_heads);
     if ((int64_t)args->batch * pool->num_kv_heads * (rows > 32 ? (rows + 63) / 64 : 1) >= 512) return 0;
-    return (size_t)args->batch * args->num_q_heads * args->q_len * 64 * (pool->head_dim + 4) * sizeof(float);
+    const size_t need = (size_t)args->batch * args->num_q_heads * args->q_len * 64 * (pool->head_dim + 4) * sizeof(float);
+    return need < ((size_t)64 << 20) ? need : (size_t)64 << 20;
   }
   if (args->work_items) return pace_paged_attn_workspace_bytes_for_parts(args->batch, args->num_q_heads, args->q_len, pool->head_dim, args->max_parts);
   return pace_paged_attn_workspace_bytes(args->batch, args->num_q_heads, args->q_len, pool->head_dim, args->max_seq_len,
