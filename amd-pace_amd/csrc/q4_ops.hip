@@ -40,8 +40,9 @@ __device__ __forceinline__ int q4_v_dim(int r) {
 
 // By position: one destination block of one (sequence, KV head).  A V dword has one writer, its block's workgroup: where the append
 // covers only some of its eight tokens it is read, changed and written back.
-// 8 prompts of 4096 tokens, 8 heads of 128: 48 us for 176 MB, 41 us with the quantising left out.  Several blocks per workgroup with
-// the next one's rows under way measured 3 .. 8 us more: eight workgroups per compute unit hide the loads already.
+// 8 prompts of 4096 tokens, 8 heads of 128, stored (176 MB) and read back (the same): 79 us, 4.5 TB/s, where a plain copy moves
+// 5.1.  Two, four or eight blocks per workgroup with the next one's rows under way took 2, 3 and 6 us more: the workgroups
+// that share a compute unit hide the loads already.  One token each of 64 sequences, stored and read back: 10 us, latency.
 template <int D>
 __global__ __launch_bounds__(2 * D) void q4_append_paged_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
                                                                 const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh, int64_t st,
@@ -152,12 +153,12 @@ __global__ __launch_bounds__(2 * D) void q4_append_slots_kernel(pace_kv_pool_t p
 // ---------------------------------------------------------------------------------
 // Read back.  One workgroup of 2 D threads rebuilds one logical block (16 tokens) of one KV head as token rows: thread
 // (token, chunk) makes eight dims of K from one code dword, and eight dims of V from the eight dwords its token has a
-// code in, which pass through LDS.
+// code in, which pass through LDS.  64 sequences of 128 .. 8192 tokens, 8 heads of 128: 136 us for 700 MB, the 5.1 TB/s of a plain copy.
 // ---------------------------------------------------------------------------------
 // packed_entry() with the owner found by the lanes of a wave side by side: 64 sequences per memory round trip where the bisection
-// takes one per step.  For grids that are on the GPU all at once, whose time is a chain of such trips (5 sequences:
-// the same 4.3 us; 64: 4.9 -> 4.0 us); a long grid hides them and pays for the vector work (130 k tokens of 64
-// sequences: 134 us by bisection, 158 us this way).
+// takes one per step.  For grids that are on the GPU all at once, whose time is a chain of such trips (one read of 64
+// short sequences, nothing of it in a cache: 8.4 us by bisection, 7.5 us this way; 5 sequences: 4.3 us either way); a long
+// grid hides them and pays for the vector work (64 sequences of 128 .. 8192 tokens: 134 us by bisection, 158 us this way).
 __device__ __forceinline__ void q4_packed_entry(const int32_t* __restrict__ cu, int batch, int H, unsigned entry, int lane, int& b, int& h, int& j) {
   for (int base = 0;; base += 64) {
     const int i = min(base + lane, batch - 1);

@@ -16,7 +16,6 @@
 #include <algorithm>
 
 #include "attn_core.h"
-#include "kv_ops.h"
 #include "q4.h"
 
 namespace pace_kv {
@@ -24,10 +23,10 @@ namespace pace_kv {
 struct WalkParams : PagedAttnParams {
   int32_t window, sinks;  // 0: off
   int32_t group_rows;     // query rows of a group
+  int32_t slot_rows;      // query rows of a partial result
   // How the groups (sequence, run of query rows) are dealt to workgroups.  shares == 0: one workgroup per group and KV head.  Else
   // the units of all groups of a KV head lie end to end and `shares` workgroups take equal runs of them (at least
-  // min_share and part_units, a multiple of min_share), so that a batch of any lengths keeps every
-  // workgroup busy for the same time.  A group that one workgroup covers alone is finished there; pieces of others
+  // min_share and part_units), so that a batch of any lengths keeps every workgroup busy for the same time.  A group that one workgroup covers alone is finished there; pieces of others
   // become partial results, two per workgroup at most -- the group it starts in the middle of or with, and the one it
   // breaks off -- which walk_merge_kernel joins.
   int32_t shares, min_share, part_units;
@@ -84,8 +83,7 @@ struct Shares {
   int total, share;
 };
 __device__ __forceinline__ int walk_share(const WalkParams& p, int total) {
-  const int share = max(max((total + p.shares - 1) / p.shares, p.min_share), p.part_units);
-  return (share + p.min_share - 1) / p.min_share * p.min_share;
+  return max(max((total + p.shares - 1) / p.shares, p.min_share), p.part_units);  // (unrounded: equal sequences stay whole)
 }
 __device__ __forceinline__ int wave_sum(int v) {
 #pragma unroll
@@ -549,7 +547,7 @@ __device__ __forceinline__ void walk_store(const WalkParams& p, const WalkRows<D
       *reinterpret_cast<u32x2*>(op + 16 * j) = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
     }
   } else {
-    const int64_t at = ((int64_t)slot * p.num_kv_heads + kvh) * p.max_parts + row;  // (max_parts: rows of a slot)
+    const int64_t at = ((int64_t)slot * p.num_kv_heads + kvh) * p.slot_rows + row;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * j + 4 * g) = st.o[qt][j];
     if (g == 0) *reinterpret_cast<u32x2*>(p.part_ml + 2 * at) = u32x2{__float_as_uint(st.m[qt]), __float_as_uint(l)};
@@ -589,8 +587,15 @@ struct WalkTurns {
 };
 
 // ---------------------------------------------------------------------------------
-// Up to 16 query rows per KV head (decode): every wave walks units of its own.  NW waves split a partition's units (wave w:
+// Up to 16 query rows per KV head (decode): every wave walks units of its own.  NW waves split a workgroup's units (wave w:
 // units w, w + NW, ...), fetch one ahead, and merge through LDS.
+//
+// Bound: the pool's bytes.  64 sequences x 4096 tokens, 8 KV heads of 128 dims, 4 query heads each: 57 us for 336 MB of
+// 4-bit rows, 5.9 TB/s, where a plain read of as much reaches 6.0; 32 sequences through a window of 4096 tokens over a bf16
+// pool: 86 us, 6.3 TB/s (a window's rows partly come from the cache).  One sequence of 4096 tokens: 10.5 us, the latency of
+// two launches and of four units one after another.  Four waves and units in turn rather than one wave per run of units: a
+// workgroup's reads stay close together.  Two waves for 256 dims, whose state takes a wave's whole register file.
+// Two or three row tiles per wave instead of walk_rows_kernel (36 rows): 123 us against 65 -- one wave per SIMD, and spills.
 // ---------------------------------------------------------------------------------
 template <int BITS, int D, bool HAS_MASK, int NW, int OCC>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8))) void walk_attn_kernel(const WalkParams p) {
@@ -609,117 +614,117 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     early = t < p.table_stride ? p.table[t] : 0;
   }
   do {
-  const Group x = walk_group(p, turns.j);
-  const int b = x.b, len = x.len, start = x.start;
-  const Walk walk = x.walk;
-  int i_begin, i_end, slot;
-  const bool some = turns.piece(x, i_begin, i_end, slot);
-  ++turns.j;
-  if (!some) continue;  // uniform over the workgroup
-  const int32_t* row = p.table + (int64_t)b * p.table_stride;
-  const int n_mine = i_end - i_begin > wave ? (i_end - i_begin - wave + NW - 1) / NW : 0;
+    const Group x = walk_group(p, turns.j);
+    const int b = x.b, len = x.len, start = x.start;
+    const Walk walk = x.walk;
+    int i_begin, i_end, slot;
+    const bool some = turns.piece(x, i_begin, i_end, slot);
+    ++turns.j;
+    if (!some) continue;  // uniform over the workgroup
+    const int32_t* row = p.table + (int64_t)b * p.table_stride;
+    const int n_mine = i_end - i_begin > wave ? (i_end - i_begin - wave + NW - 1) / NW : 0;
 
-  // Pool block ids of 32 units of this wave, one per lane; never outside the pool, whatever the table holds.
-  auto inside = [&](int id) { return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id); };
-  auto fetch_ids = [&](int first) {
-    const int i = i_begin + wave + NW * (first + (lane >> 1));
-    const int t = 2 * walk.unit(i) + (lane & 1);
-    return inside(i < i_end && t < p.table_stride ? row[t] : 0);
-  };
-  int ids = known ? inside(early) : (n_mine > 0 ? fetch_ids(0) : 0);
-  const LaneBase base = WalkUnit<BITS, D>::base(p, kvh, n, g);
-  constexpr bool TWO = !(D == 256 && (BITS == 16 || HAS_MASK));  // registers for a second unit under way
-  WalkUnit<BITS, D> even, odd;
-  MaskRaw<1> even_mask, odd_mask;  // mask values travel with the unit, ahead of it
-  const int64_t mask_line[1] = {HAS_MASK ? walk_mask_line(p, b, n) : 0};
-  if constexpr (BITS == 4) even.or_bits = odd.or_bits = q4_or_bits();
-  auto send = [&](WalkUnit<BITS, D>& u, MaskRaw<1>& m, int k) {
-    if (HAS_MASK) load_mask_raw<1>(m, p, mask_line, 32 * walk.unit(i_begin + wave + NW * k), g);
-    u.load(base, unit_offsets<BITS>(p, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1)), n, g);
-  };
-  if (n_mine > 0) send(even, even_mask, 0);
+    // Pool block ids of 32 units of this wave, one per lane; never outside the pool, whatever the table holds.
+    auto inside = [&](int id) { return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id); };
+    auto fetch_ids = [&](int first) {
+      const int i = i_begin + wave + NW * (first + (lane >> 1));
+      const int t = 2 * walk.unit(i) + (lane & 1);
+      return inside(i < i_end && t < p.table_stride ? row[t] : 0);
+    };
+    int ids = known ? inside(early) : (n_mine > 0 ? fetch_ids(0) : 0);
+    const LaneBase base = WalkUnit<BITS, D>::base(p, kvh, n, g);
+    constexpr bool TWO = !(D == 256 && (BITS == 16 || HAS_MASK));  // registers for a second unit under way
+    WalkUnit<BITS, D> even, odd;
+    MaskRaw<1> even_mask, odd_mask;  // mask values travel with the unit, ahead of it
+    const int64_t mask_line[1] = {HAS_MASK ? walk_mask_line(p, b, n) : 0};
+    if constexpr (BITS == 4) even.or_bits = odd.or_bits = q4_or_bits();
+    auto send = [&](WalkUnit<BITS, D>& u, MaskRaw<1>& m, int k) {
+      if (HAS_MASK) load_mask_raw<1>(m, p, mask_line, 32 * walk.unit(i_begin + wave + NW * k), g);
+      u.load(base, unit_offsets<BITS>(p, __builtin_amdgcn_readlane(ids, 2 * (k & 31)), __builtin_amdgcn_readlane(ids, 2 * (k & 31) + 1)), n, g);
+    };
+    if (n_mine > 0) send(even, even_mask, 0);
 
-  WalkRows<D, 1> st;
-  int min_limit = walk_row<BITS, D, 1, HAS_MASK>(p, st, 0, b, kvh, len, n, g);
+    WalkRows<D, 1> st;
+    int min_limit = walk_row<BITS, D, 1, HAS_MASK>(p, st, 0, b, kvh, len, n, g);
 #pragma unroll
-  for (int o = 1; o < 16; o *= 2) min_limit = min(min_limit, __shfl_xor(min_limit, o, 64));
-  min_limit = __builtin_amdgcn_readfirstlane(min_limit);
-  const int row_low = p.window > 0 ? len - S - p.window + 1 : 0;  // the first row's window, and the last row's
-  const int max_low = p.window > 0 ? len - p.window : 0;
+    for (int o = 1; o < 16; o *= 2) min_limit = min(min_limit, __shfl_xor(min_limit, o, 64));
+    min_limit = __builtin_amdgcn_readfirstlane(min_limit);
+    const int row_low = p.window > 0 ? len - S - p.window + 1 : 0;  // the first row's window, and the last row's
+    const int max_low = p.window > 0 ? len - p.window : 0;
 
-  auto take = [&](WalkUnit<BITS, D>& u, const MaskRaw<1>& m, int k) {
-    const int t0 = 32 * walk.unit(i_begin + wave + NW * k);
-    MaskRegs<1> mregs;
-    if (HAS_MASK) {
-      mask_regs_from_raw<1>(mregs, m, p);
-      if (walk_masked_out<D, 1>(mregs, st)) return;
-    }
-    const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
-    if (BITS == 16 && !full) u.drop(walk_keep(t0, g, start, walk.sink_end, row_low, len));
-    f32x4 sc[1][2];
-    u32x4 pb[1];
-    walk_scores<BITS, D, 1, 1>([&](int t, int kk) { return u.k(t, kk); }, st, sc);
-    walk_weights<BITS, D, 1, HAS_MASK>(sc, st, pb, full, t0, start, walk.sink_end, g, mregs);
-    walk_output<BITS, D, 1, 1>([&](int j) { return u.v(j); }, st, pb);
-  };
-  // 32 units per set of block ids.  (Every turn of the inner loop fetches: behind a fetch that may or may not have been sent, the
-  // compiler would have the wave wait for all that is under way before it uses the unit before it.)
-  for (int k0 = 0; k0 < n_mine; k0 += 32) {
-    const int k1 = min(k0 + 32, n_mine);
-    if (k0 > 0) {
-      ids = fetch_ids(k0);
-      send(even, even_mask, k0);
-    }
-    int k = k0;
-    if constexpr (TWO) {
-      for (; k + 2 < k1; k += 2) {
-        send(odd, odd_mask, k + 1);
-        take(even, even_mask, k);
-        send(even, even_mask, k + 2);
-        take(odd, odd_mask, k + 1);
+    auto take = [&](WalkUnit<BITS, D>& u, const MaskRaw<1>& m, int k) {
+      const int t0 = 32 * walk.unit(i_begin + wave + NW * k);
+      MaskRegs<1> mregs;
+      if (HAS_MASK) {
+        mask_regs_from_raw<1>(mregs, m, p);
+        if (walk_masked_out<D, 1>(mregs, st)) return;
       }
-      if (k + 1 < k1) {
-        send(odd, odd_mask, k + 1);
-        take(even, even_mask, k);
-        take(odd, odd_mask, k + 1);
+      const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
+      if (BITS == 16 && !full) u.drop(walk_keep(t0, g, start, walk.sink_end, row_low, len));
+      f32x4 sc[1][2];
+      u32x4 pb[1];
+      walk_scores<BITS, D, 1, 1>([&](int t, int kk) { return u.k(t, kk); }, st, sc);
+      walk_weights<BITS, D, 1, HAS_MASK>(sc, st, pb, full, t0, start, walk.sink_end, g, mregs);
+      walk_output<BITS, D, 1, 1>([&](int j) { return u.v(j); }, st, pb);
+    };
+    // 32 units per set of block ids.  (Every turn of the inner loop fetches: behind a fetch that may or may not have been sent, the
+    // compiler would have the wave wait for all that is under way before it uses the unit before it.)
+    for (int k0 = 0; k0 < n_mine; k0 += 32) {
+      const int k1 = min(k0 + 32, n_mine);
+      if (k0 > 0) {
+        ids = fetch_ids(k0);
+        send(even, even_mask, k0);
+      }
+      int k = k0;
+      if constexpr (TWO) {
+        for (; k + 2 < k1; k += 2) {
+          send(odd, odd_mask, k + 1);
+          take(even, even_mask, k);
+          send(even, even_mask, k + 2);
+          take(odd, odd_mask, k + 1);
+        }
+        if (k + 1 < k1) {
+          send(odd, odd_mask, k + 1);
+          take(even, even_mask, k);
+          take(odd, odd_mask, k + 1);
+        } else {
+          take(even, even_mask, k);
+        }
       } else {
+        for (; k + 1 < k1; ++k) {
+          take(even, even_mask, k);
+          send(even, even_mask, k + 1);
+        }
         take(even, even_mask, k);
       }
-    } else {
-      for (; k + 1 < k1; ++k) {
-        take(even, even_mask, k);
-        send(even, even_mask, k + 1);
+    }
+    walk_finish<D, 1, HAS_MASK>(st);
+    // Pairwise merge of the waves' states (fixed order: the same bits from call to call).
+#pragma unroll
+    for (int stride = 1; stride < NW; stride *= 2) {
+      float* slot = merge_buf + wave / (2 * stride) * SLOT_F + n * ROW_F;
+      const bool sender = (wave & (2 * stride - 1)) == stride, receiver = (wave & (2 * stride - 1)) == 0;
+      if (sender) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) slot[16 * j + 4 * g + i] = st.o[0][j][i];
+        if (g == 0) slot[D] = st.m[0], slot[D + 1] = st.sum[0][0];
       }
-      take(even, even_mask, k);
+      __syncthreads();
+      if (receiver) {
+        const float m_b = slot[D], l_b = slot[D + 1], m_new = fmaxf(st.m[0], m_b), m_use = m_new == kNegInf ? 0.f : m_new;
+        const float wa = __builtin_amdgcn_exp2f(st.m[0] - m_use), wb = __builtin_amdgcn_exp2f(m_b - m_use);
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.o[0][j][i] = st.o[0][j][i] * wa + slot[16 * j + 4 * g + i] * wb;
+        st.sum[0][0] = st.sum[0][0] * wa + l_b * wb;
+        st.m[0] = m_new;
+      }
+      __syncthreads();
     }
-  }
-  walk_finish<D, 1, HAS_MASK>(st);
-  // Pairwise merge of the waves' states (fixed order: the same bits from call to call).
-#pragma unroll
-  for (int stride = 1; stride < NW; stride *= 2) {
-    float* slot = merge_buf + wave / (2 * stride) * SLOT_F + n * ROW_F;
-    const bool sender = (wave & (2 * stride - 1)) == stride, receiver = (wave & (2 * stride - 1)) == 0;
-    if (sender) {
-#pragma unroll
-      for (int j = 0; j < MT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) slot[16 * j + 4 * g + i] = st.o[0][j][i];
-      if (g == 0) slot[D] = st.m[0], slot[D + 1] = st.sum[0][0];
-    }
-    __syncthreads();
-    if (receiver) {
-      const float m_b = slot[D], l_b = slot[D + 1], m_new = fmaxf(st.m[0], m_b), m_use = m_new == kNegInf ? 0.f : m_new;
-      const float wa = __builtin_amdgcn_exp2f(st.m[0] - m_use), wb = __builtin_amdgcn_exp2f(m_b - m_use);
-#pragma unroll
-      for (int j = 0; j < MT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[0][j][i] = st.o[0][j][i] * wa + slot[16 * j + 4 * g + i] * wb;
-      st.sum[0][0] = st.sum[0][0] * wa + l_b * wb;
-      st.m[0] = m_new;
-    }
-    __syncthreads();
-  }
-  if (wave == 0 && n < R) walk_store(p, st, 0, b, kvh, slot, n, g);
+    if (wave == 0 && n < R) walk_store(p, st, 0, b, kvh, slot, n, g);
   } while (p.shares > 0 && turns.left > 0 && turns.j < n_groups);
 }
 
@@ -728,6 +733,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
 // units together.  Each wave fetches and unpacks a quarter of a unit and puts it into LDS in operand order, so that the
 // unpacking is paid once per workgroup; fetches run three units ahead of their use (two in registers, one in LDS), with
 // one barrier per unit.  A row's softmax state never leaves its wave.
+//
+// Bound: issue.  Matrix and vector instructions of the waves of one SIMD do not overlap, and per 32 tokens and tile 18 matrix
+// instructions (128 dims) stand next to some 60 vector ones (softmax, and a quarter of the unpacking).  4 sequences x 512 new
+// tokens over 4096 (8 KV heads of 128 dims, 4 query heads each): 170 us, 760 TFLOP/s, where a large fp16 matrix product
+// reaches 1200; the same with every wave unpacking for itself: 330 us.  32 sequences x 9 drafted tokens over 1000 .. 6000:
+// 65 us for 70 MB of rows, in which 36 of the 64 rows a workgroup computes are real.  Two tiles per wave above 64 rows halve
+// the LDS reads and the unpacking per row; with a mask tensor some registers spill at 128 dims, which costs less than twice as
+// many workgroups would.  Workgroups per compute unit under one tile, drafted tokens: 2 / 3 / 4 run 79 / 72 / 84 us.
 // ---------------------------------------------------------------------------------
 template <int BITS, int D, int NQT, bool HAS_MASK, int OCC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) void walk_rows_kernel(const WalkParams p) {
@@ -738,132 +751,133 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
   WalkTurns turns(p, lane);
   const int kvh = turns.kvh, S = p.q_len, R = S * p.n_rep, n_groups = p.batch * p.n_qgroups;
   do {
-  const Group x = walk_group(p, turns.j);
-  const int b = x.b, len = x.len, start = x.start, r_first = x.r_first;
-  const Walk walk = x.walk;
-  int i_begin, i_end, slot;
-  const bool some = turns.piece(x, i_begin, i_end, slot);
-  ++turns.j;
-  if (!some) continue;  // uniform over the workgroup
-  const int wg_low = p.window > 0 ? len - S + x.s_first - p.window + 1 : 0;  // what no row of the workgroup reads (see walk_keep)
-  const int wg_end = p.causal ? min(len, len - S + x.s_last + 1) : len;
+    const Group x = walk_group(p, turns.j);
+    const int b = x.b, len = x.len, start = x.start, r_first = x.r_first;
+    const Walk walk = x.walk;
+    int i_begin, i_end, slot;
+    const bool some = turns.piece(x, i_begin, i_end, slot);
+    ++turns.j;
+    if (!some) continue;  // uniform over the workgroup
+    const int wg_low = p.window > 0 ? len - S + x.s_first - p.window + 1 : 0;  // what no row of the workgroup reads (see walk_keep)
+    const int wg_end = p.causal ? min(len, len - S + x.s_last + 1) : len;
 
-  const int32_t* row = p.table + (int64_t)b * p.table_stride;
-  // Pool blocks of 64 units from c0 on, one per lane in each of two registers; never outside the pool.
-  auto fetch_id = [&](int i) {
-    const int t = 2 * walk.unit(i) + (lane & 1);
-    const int id = i < i_end && t < p.table_stride ? row[t] : 0;
-    return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
-  };
-  int c0 = i_begin, ids_lo = fetch_id(c0 + (lane >> 1)), ids_hi = fetch_id(c0 + 32 + (lane >> 1));
-  const LaneBase base = UnitShare<BITS, D>::base(p, kvh, wave, n, g);
-  const uint32_t or_bits = q4_or_bits();
-  UnitShare<BITS, D> even, odd;
-  auto send = [&](UnitShare<BITS, D>& share, int i) {
-    const int at = 2 * (i - c0);  // (past the 64 units: whatever block the lane holds; nobody reads that share)
-    const int idA = at & 64 ? __builtin_amdgcn_readlane(ids_hi, at & 63) : __builtin_amdgcn_readlane(ids_lo, at & 63);
-    const int idB = at & 64 ? __builtin_amdgcn_readlane(ids_hi, (at & 63) + 1) : __builtin_amdgcn_readlane(ids_lo, (at & 63) + 1);
-    share.load(base, unit_offsets<BITS>(p, idA, idB), wave, n, g);
-  };
-  auto put = [&](UnitShare<BITS, D>& share, int i) {  // (past the last unit: whatever the share holds, into a stage nobody reads)
-    u32x4 keep = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-    if (BITS == 16) {
+    const int32_t* row = p.table + (int64_t)b * p.table_stride;
+    // Pool blocks of 64 units from c0 on, one per lane in each of two registers; never outside the pool.
+    auto fetch_id = [&](int i) {
+      const int t = 2 * walk.unit(i) + (lane & 1);
+      const int id = i < i_end && t < p.table_stride ? row[t] : 0;
+      return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : id);
+    };
+    int c0 = i_begin, ids_lo = fetch_id(c0 + (lane >> 1)), ids_hi = fetch_id(c0 + 32 + (lane >> 1));
+    const LaneBase base = UnitShare<BITS, D>::base(p, kvh, wave, n, g);
+    const uint32_t or_bits = q4_or_bits();
+    UnitShare<BITS, D> even, odd;
+    auto send = [&](UnitShare<BITS, D>& share, int i) {
+      const int at = 2 * (i - c0);  // (past the 64 units: whatever block the lane holds; nobody reads that share)
+      const int idA = at & 64 ? __builtin_amdgcn_readlane(ids_hi, at & 63) : __builtin_amdgcn_readlane(ids_lo, at & 63);
+      const int idB = at & 64 ? __builtin_amdgcn_readlane(ids_hi, (at & 63) + 1) : __builtin_amdgcn_readlane(ids_lo, (at & 63) + 1);
+      share.load(base, unit_offsets<BITS>(p, idA, idB), wave, n, g);
+    };
+    auto put = [&](UnitShare<BITS, D>& share, int i) {  // (past the last unit: whatever the share holds, into a stage nobody reads)
+      u32x4 keep = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+      if (BITS == 16) {
+        const int t0 = 32 * walk.unit(i);
+        if (t0 < start || t0 + 32 > wg_end || t0 < wg_low) keep = walk_keep(t0, g, start, walk.sink_end, wg_low, wg_end);
+      }
+      share.put(stage[(i - c0) & 1], wave, lane, keep, or_bits);
+    };
+    send(even, c0);
+    send(odd, c0 + 1);
+
+    WalkRows<D, NQT> st;
+    const int w_first = r_first + wave * NQT * 16, w_last = min(R, w_first + NQT * 16) - 1;  // this wave's rows
+    const bool any_rows = w_first < R;
+    int min_limit = 0x7fffffff;
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) min_limit = min(min_limit, walk_row<BITS, D, NQT, HAS_MASK>(p, st, qt, b, kvh, len, w_first + qt * 16 + n, g));
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) min_limit = min(min_limit, __shfl_xor(min_limit, o, 64));
+    min_limit = __builtin_amdgcn_readfirstlane(min_limit);
+    const int row_low = p.window > 0 ? len - S + w_first / p.n_rep - p.window + 1 : 0;
+    const int max_low = p.window > 0 ? len - S + w_last / p.n_rep - p.window + 1 : 0;
+    const int row_end = !any_rows ? 0 : (p.causal ? min(len, len - S + w_last / p.n_rep + 1) : len);
+
+    // One turn: unit i + 1 of the set goes from `next` into LDS, `next` fetches unit i + 3, unit i is used.  With two tiles per wave LDS
+    // reads travel behind vector work: the K operands are asked for before the unpacking, the V operands before the softmax
+    // that needs them after it.  (With one tile a third workgroup on the compute unit does that, and registers are kept for
+    // it; head size 256 and a mask have none to spare.)  At the barrier every wave has taken what it needs of unit i, and every share of
+    // unit i + 1 is in place.
+    constexpr bool AHEAD = D <= 128 && NQT == 2 && !HAS_MASK;
+    constexpr int CHUNK = AHEAD ? 1 : (NQT == 2 ? 4 : 8);
+    MaskRaw<NQT> coming;  // mask values of the next unit: asked for a turn ahead, before that turn's share
+    int64_t mask_line[NQT];
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) mask_line[qt] = HAS_MASK ? walk_mask_line(p, b, w_first + qt * 16 + n) : 0;
+    auto turn = [&](UnitShare<BITS, D>& next, int i) {
       const int t0 = 32 * walk.unit(i);
-      if (t0 < start || t0 + 32 > wg_end || t0 < wg_low) keep = walk_keep(t0, g, start, walk.sink_end, wg_low, wg_end);
-    }
-    share.put(stage[(i - c0) & 1], wave, lane, keep, or_bits);
-  };
-  send(even, c0);
-  send(odd, c0 + 1);
-
-  WalkRows<D, NQT> st;
-  const int w_first = r_first + wave * NQT * 16, w_last = min(R, w_first + NQT * 16) - 1;  // this wave's rows
-  const bool any_rows = w_first < R;
-  int min_limit = 0x7fffffff;
-#pragma unroll
-  for (int qt = 0; qt < NQT; ++qt) min_limit = min(min_limit, walk_row<BITS, D, NQT, HAS_MASK>(p, st, qt, b, kvh, len, w_first + qt * 16 + n, g));
-#pragma unroll
-  for (int o = 1; o < 16; o *= 2) min_limit = min(min_limit, __shfl_xor(min_limit, o, 64));
-  min_limit = __builtin_amdgcn_readfirstlane(min_limit);
-  const int row_low = p.window > 0 ? len - S + w_first / p.n_rep - p.window + 1 : 0;
-  const int max_low = p.window > 0 ? len - S + w_last / p.n_rep - p.window + 1 : 0;
-  const int row_end = !any_rows ? 0 : (p.causal ? min(len, len - S + w_last / p.n_rep + 1) : len);
-
-  // One turn: unit i + 1 of the set goes from `next` into LDS, `next` fetches unit i + 3, unit i is used.  With two tiles per wave LDS
-  // reads travel behind vector work: the K operands are asked for before the unpacking, the V operands before the softmax
-  // that needs them after it.  (With one tile a third workgroup on the compute unit does that, and registers are kept for
-  // it; head size 256 and a mask have none to spare.)  At the barrier every wave has taken what it needs of unit i, and every share of
-  // unit i + 1 is in place.
-  constexpr bool AHEAD = D <= 128 && NQT == 2 && !HAS_MASK;
-  constexpr int CHUNK = AHEAD ? 1 : (NQT == 2 ? 4 : 8);
-  MaskRaw<NQT> coming;  // mask values of the next unit: asked for a turn ahead, before that turn's share
-  int64_t mask_line[NQT];
-#pragma unroll
-  for (int qt = 0; qt < NQT; ++qt) mask_line[qt] = HAS_MASK ? walk_mask_line(p, b, w_first + qt * 16 + n) : 0;
-  auto turn = [&](UnitShare<BITS, D>& next, int i) {
-    const int t0 = 32 * walk.unit(i);
-    const u32x4* unit = &stage[(i - c0) & 1][lane];
-    u32x4 kop[AHEAD ? 2 : 1][AHEAD ? KK : 1], vop[AHEAD ? MT : 1];
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) kop[t][kk] = unit[(t * KK + kk) * 64];
-    }
-    put(next, i + 1);
-    bool needed = t0 < row_end && (t0 + 32 > row_low || t0 < walk.sink_end);
-    MaskRegs<NQT> mregs;
-    if (HAS_MASK) {
-      mask_regs_from_raw<NQT>(mregs, coming, p);
-      load_mask_raw<NQT>(coming, p, mask_line, 32 * walk.unit(i + 1), g);
-      needed = needed && !walk_masked_out<D, NQT>(mregs, st);
-    }
-    send(next, i + 3);
-    if (needed) {
-      const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
-      f32x4 sc[NQT][2];
-      u32x4 pb[NQT];
-      walk_scores<BITS, D, NQT, CHUNK>([&](int t, int kk) { return AHEAD ? kop[AHEAD ? t : 0][AHEAD ? kk : 0] : unit[(t * KK + kk) * 64]; }, st, sc);
+      const u32x4* unit = &stage[(i - c0) & 1][lane];
+      u32x4 kop[AHEAD ? 2 : 1][AHEAD ? KK : 1], vop[AHEAD ? MT : 1];
       if constexpr (AHEAD) {
 #pragma unroll
-        for (int j = 0; j < MT; ++j) vop[j] = unit[(MT + j) * 64];
-      }
-      walk_weights<BITS, D, NQT, HAS_MASK>(sc, st, pb, full, t0, start, walk.sink_end, g, mregs);
-      walk_output<BITS, D, NQT, CHUNK>([&](int j) { return AHEAD ? vop[AHEAD ? j : 0] : unit[(MT + j) * 64]; }, st, pb);
-    }
-    __syncthreads();
-  };
-  // 64 units per set of block ids.  (Every turn of the inner loop fetches, past the last unit block 0 of the pool, which nobody reads:
-  // behind a fetch that may or may not have been sent, the compiler would have the wave wait for all that is under way
-  // before it uses the share before it.)
-  for (; c0 < i_end; c0 += 64) {
-    if (c0 > i_begin) {
-      ids_lo = fetch_id(c0 + (lane >> 1)), ids_hi = fetch_id(c0 + 32 + (lane >> 1));
-      send(even, c0);
-      send(odd, c0 + 1);
-    }
-    const int c1 = min(c0 + 64, i_end);
-    put(even, c0);
-    if (HAS_MASK) load_mask_raw<NQT>(coming, p, mask_line, 32 * walk.unit(c0), g);
-    send(even, c0 + 2);
-    __syncthreads();
-    int i = c0;
-    for (; i + 1 < c1; i += 2) {
-      turn(odd, i);
-      turn(even, i + 1);
-    }
-    if (i < c1) turn(odd, i);
-  }
-  walk_finish<D, NQT, HAS_MASK>(st);
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-  for (int qt = 0; qt < NQT; ++qt)
-    if (w_first + qt * 16 + n < R) walk_store(p, st, qt, b, kvh, slot, w_first + qt * 16 + n - r_first, g);
+          for (int kk = 0; kk < KK; ++kk) kop[t][kk] = unit[(t * KK + kk) * 64];
+      }
+      put(next, i + 1);
+      bool needed = t0 < row_end && (t0 + 32 > row_low || t0 < walk.sink_end);
+      MaskRegs<NQT> mregs;
+      if (HAS_MASK) {
+        mask_regs_from_raw<NQT>(mregs, coming, p);
+        load_mask_raw<NQT>(coming, p, mask_line, 32 * walk.unit(i + 1), g);
+        needed = needed && !walk_masked_out<D, NQT>(mregs, st);
+      }
+      send(next, i + 3);
+      if (needed) {
+        const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
+        f32x4 sc[NQT][2];
+        u32x4 pb[NQT];
+        walk_scores<BITS, D, NQT, CHUNK>([&](int t, int kk) { return AHEAD ? kop[AHEAD ? t : 0][AHEAD ? kk : 0] : unit[(t * KK + kk) * 64]; }, st, sc);
+        if constexpr (AHEAD) {
+#pragma unroll
+          for (int j = 0; j < MT; ++j) vop[j] = unit[(MT + j) * 64];
+        }
+        walk_weights<BITS, D, NQT, HAS_MASK>(sc, st, pb, full, t0, start, walk.sink_end, g, mregs);
+        walk_output<BITS, D, NQT, CHUNK>([&](int j) { return AHEAD ? vop[AHEAD ? j : 0] : unit[(MT + j) * 64]; }, st, pb);
+      }
+      __syncthreads();
+    };
+    // 64 units per set of block ids.  (Every turn of the inner loop fetches, past the last unit block 0 of the pool, which nobody reads:
+    // behind a fetch that may or may not have been sent, the compiler would have the wave wait for all that is under way
+    // before it uses the share before it.)
+    for (; c0 < i_end; c0 += 64) {
+      if (c0 > i_begin) {
+        ids_lo = fetch_id(c0 + (lane >> 1)), ids_hi = fetch_id(c0 + 32 + (lane >> 1));
+        send(even, c0);
+        send(odd, c0 + 1);
+      }
+      const int c1 = min(c0 + 64, i_end);
+      put(even, c0);
+      if (HAS_MASK) load_mask_raw<NQT>(coming, p, mask_line, 32 * walk.unit(c0), g);
+      send(even, c0 + 2);
+      __syncthreads();
+      int i = c0;
+      for (; i + 1 < c1; i += 2) {
+        turn(odd, i);
+        turn(even, i + 1);
+      }
+      if (i < c1) turn(odd, i);
+    }
+    walk_finish<D, NQT, HAS_MASK>(st);
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt)
+      if (w_first + qt * 16 + n < R) walk_store(p, st, qt, b, kvh, slot, w_first + qt * 16 + n - r_first, g);
   } while (p.shares > 0 && turns.left > 0 && turns.j < n_groups);
 }
 
 // out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partial results of a query row.  A wave takes eight at a time, a lane the
 // dims 2 lane, 2 lane + 1 (+ 128); WPR waves share a row (partial results in turn, joined through LDS).  Rows of groups that
 // one workgroup covered are finished already; rows that read nothing belong to no workgroup and become 0 here.
+// Bound: latency (a launch, the lengths, then the partial results): some 5 us next to one sequence, up to 10 next to 9216 rows.
 template <int D, int WPR>
 __global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int32_t total_rows) {
   constexpr int PASSES = (D + 127) / 128;
@@ -892,7 +906,7 @@ __global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int
   if (n_parts == 1) return;  // uniform over the row's waves
   // workgroup w0 + i's piece lies in its first slot, except the first one's if that workgroup began with other groups
   const int late = at % share != 0 ? 1 : 0;
-  auto place = [&](int i) { return ((int64_t)(2 * (w0 + i) + (i == 0 ? late : 0)) * p.num_kv_heads + kvh) * p.max_parts + (r - qg * p.group_rows); };
+  auto place = [&](int i) { return ((int64_t)(2 * (w0 + i) + (i == 0 ? late : 0)) * p.num_kv_heads + kvh) * p.slot_rows + (r - qg * p.group_rows); };
   const int d0 = 2 * lane;
   float acc[PASSES][2], M = kNegInf, L = 0.f;
 #pragma unroll
@@ -976,25 +990,38 @@ static WalkShape walk_shape(const pace_kv_pool_t* pool, const pace_paged_attn_ar
   s.n_qgroups = (int)((rows + s.group_rows - 1) / s.group_rows);
   s.slot_rows = (int)std::min<int64_t>(rows, s.group_rows);
   int64_t units = ((int64_t)a->max_seq_len + 31) / 32;  // of the longest group
-  if (a->window > 0) units = std::min(units, ((int64_t)a->window + a->q_len) / 32 + 2 + a->sinks / 32 + 2);
+  if (a->window > 0) {
+    const int64_t n_rep = rows / std::max(a->q_len, 1), tokens = std::min<int64_t>(a->q_len, (s.slot_rows - 1) / std::max<int64_t>(n_rep, 1) + 2);
+    units = std::min(units, (a->window + (a->causal ? tokens : a->q_len)) / 32 + 2 + a->sinks / 32 + 2);
+  }
   units = std::max<int64_t>(units, 1);
   s.min_share = s.nqt == 0 ? walk_waves(D) : 1;  // units a workgroup works on side by side
   const int64_t n_groups = (int64_t)a->batch * s.n_qgroups, groups = n_groups * heads;
-  // Workgroups that run side by side.  One per compute unit is enough for walk_attn_kernel, whose waves fetch ahead.
+  // Workgroups that run side by side and keep the GPU busy.  One per compute unit nearly is enough for walk_attn_kernel, whose
+  // waves fetch ahead; where its units are shared out it gets two (64 x 500 .. 8000 tokens: 71 us with one, 60 with two).
   const int64_t slots = (int64_t)compute_units() * (s.nqt == 0 ? 1 : rows_occ(D, s.nqt));
   int64_t shares = 0;
-  if (a->partition_tokens > 0) {
+  if (n_groups * units >= (int64_t)1 << 30) {
+    // (the run of all units is counted in 32 bits; as many groups as that need no sharing)
+  } else if (a->partition_tokens > 0) {
     s.part_units = (a->partition_tokens / 32 + s.min_share - 1) / s.min_share * s.min_share;
     shares = n_groups == 1 ? (units + s.part_units - 1) / s.part_units : (n_groups * units + s.part_units - 1) / s.part_units;
     if (units <= s.part_units && n_groups == 1) shares = 0;
   } else {
-    // Sharing costs a second launch and a trip of the partial results, some 5 us: not for groups of few units.  It pays where a
-    // workgroup per group would leave much of the GPU idle -- in its last round, or because some sequence may be far
-    // longer than the others (lengths are not known here, only their bound).
+    // Sharing costs a second launch and a trip of the partial results.  It pays where a workgroup per group would leave much of the
+    // GPU idle: throughout, in its last round, or because some sequence may be far longer than the others (lengths are not
+    // known here, only their bound).  Measured without -> with, 8 KV heads of 128 dims, 4 query heads each, us:
+    //   one row, 1 x 4096 tokens: 28 -> 10.5; 33 x 8000: 99 -> 73; 64 x 500 .. 8000: 76 -> 60; 64 x 8000: 113 -> 127;
+    //     256 x 100 .. 8000: 154 -> 175; through a window of 4096, 32 sequences: 83 -> 91
+    //   9 drafted tokens, 32 x 1000 .. 6000: 146 -> 64; 96 x 500 .. 8000: 224 -> 148; 192 x 500 .. 8000: 350 -> 302; 192 x 6000: 535 -> 534
+    //   chunks of 512, 2 x 8000: 266 -> 223; 4 x 8000: 392 -> 425; 4 x 800 .. 8000: 269 -> 313; 9 x 8000: 774 -> 852
+    // so: where less than a round of workgroups is there, and, where each has a sequence of its own, up to the rounds after which
+    // unequal lengths even out by themselves.  Not for groups of few units: they end before a second launch does.
     const double idle = (double)((groups + slots - 1) / slots * slots) / (double)groups;
     const int64_t few = s.nqt == 0 ? 8 : 16;
-    if (units > few && (units > 160 || idle > 1.2)) {
-      shares = std::max<int64_t>(slots / heads, 1);
+    const bool own_sequence = s.n_qgroups == 1 && groups <= slots * (s.nqt == 0 ? 4 : 2);
+    if (units > few && ((groups < slots && idle > 1.2) || (own_sequence && (units > 160 || idle > 1.2)))) {
+      shares = std::max<int64_t>((s.nqt == 0 ? 2 : 1) * slots / heads, 1);
       if (s.nqt != 0) s.min_share = 4;
       if (n_groups == 1) {
         s.part_units = (int)std::max<int64_t>((units + shares - 1) / shares, s.nqt == 0 ? 4 : 12);
@@ -1057,7 +1084,7 @@ int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, con
   p.causal = a->causal;
   p.scale = a->scale, p.scale_log2 = a->scale * kLog2e;
   p.window = std::min(a->window, 1 << 30), p.sinks = std::min(a->sinks, 1 << 30);  // (sums with them stay below 2^31)
-  p.n_qgroups = sh.n_qgroups, p.group_rows = sh.group_rows, p.max_parts = sh.slot_rows;
+  p.n_qgroups = sh.n_qgroups, p.group_rows = sh.group_rows, p.slot_rows = sh.slot_rows;
   p.shares = sh.shares, p.min_share = sh.min_share, p.part_units = sh.part_units;
   const size_t rows = (size_t)a->batch * a->num_q_heads * a->q_len;
   PACE_REQUIRE(rows < ((size_t)1 << 31), "%s: too many query rows", who);
