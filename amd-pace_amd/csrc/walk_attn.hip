@@ -587,7 +587,7 @@ struct WalkTurns {
 };
 
 // ---------------------------------------------------------------------------------
-// Up to 16 query rows per KV head (decode): every wave walks units of its own.  NW waves split a workgroup's units (wave w:
+// Groups of up to 16 query rows (decode; short appends, and prompts too short to fill the GPU otherwise): every wave walks units of its own.  NW waves split a workgroup's units (wave w:
 // units w, w + NW, ...), fetch one ahead, and merge through LDS.
 //
 // Bound: the pool's bytes.  64 sequences x 4096 tokens, 8 KV heads of 128 dims, 4 query heads each: 57 us for 336 MB of
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     constexpr bool TWO = !(D == 256 && (BITS == 16 || HAS_MASK));  // registers for a second unit under way
     WalkUnit<BITS, D> even, odd;
     MaskRaw<1> even_mask, odd_mask;  // mask values travel with the unit, ahead of it
-    const int64_t mask_line[1] = {HAS_MASK ? walk_mask_line(p, b, n) : 0};
+    const int64_t mask_line[1] = {HAS_MASK ? walk_mask_line(p, b, x.r_first + n) : 0};
     if constexpr (BITS == 4) even.or_bits = odd.or_bits = q4_or_bits();
     auto send = [&](WalkUnit<BITS, D>& u, MaskRaw<1>& m, int k) {
       if (HAS_MASK) load_mask_raw<1>(m, p, mask_line, 32 * walk.unit(i_begin + wave + NW * k), g);
@@ -645,12 +645,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     if (n_mine > 0) send(even, even_mask, 0);
 
     WalkRows<D, 1> st;
-    int min_limit = walk_row<BITS, D, 1, HAS_MASK>(p, st, 0, b, kvh, len, n, g);
+    int min_limit = walk_row<BITS, D, 1, HAS_MASK>(p, st, 0, b, kvh, len, x.r_first + n, g);
 #pragma unroll
     for (int o = 1; o < 16; o *= 2) min_limit = min(min_limit, __shfl_xor(min_limit, o, 64));
     min_limit = __builtin_amdgcn_readfirstlane(min_limit);
-    const int row_low = p.window > 0 ? len - S - p.window + 1 : 0;  // the first row's window, and the last row's
-    const int max_low = p.window > 0 ? len - p.window : 0;
+    const int row_low = p.window > 0 ? len - S + x.s_first - p.window + 1 : 0;  // the first row's window, and the last row's
+    const int max_low = p.window > 0 ? len - S + x.s_last - p.window + 1 : 0;
 
     auto take = [&](WalkUnit<BITS, D>& u, const MaskRaw<1>& m, int k) {
       const int t0 = 32 * walk.unit(i_begin + wave + NW * k);
@@ -724,12 +724,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
       }
       __syncthreads();
     }
-    if (wave == 0 && n < R) walk_store(p, st, 0, b, kvh, slot, n, g);
+    if (wave == 0 && x.r_first + n < R) walk_store(p, st, 0, b, kvh, slot, n, g);
   } while (p.shares > 0 && turns.left > 0 && turns.j < n_groups);
 }
 
 // ---------------------------------------------------------------------------------
-// More query rows (drafted tokens, chunks of a prompt): the four waves of a workgroup own NQT tiles of 16 rows each and walk the
+// Groups of 64 or 128 query rows (drafted tokens, chunks of a prompt): the four waves of a workgroup own NQT tiles of 16 rows each and walk the
 // units together.  Each wave fetches and unpacks a quarter of a unit and puts it into LDS in operand order, so that the
 // unpacking is paid once per workgroup; fetches run three units ahead of their use (two in registers, one in LDS), with
 // one barrier per unit.  A row's softmax state never leaves its wave.
@@ -973,6 +973,7 @@ struct WalkShape {
   int group_rows;  // query rows per group
   int n_qgroups, shares, min_share, part_units;  // see WalkParams
   int slot_rows;   // rows of a partial result
+  int64_t units;   // of the longest group
   size_t bytes;    // of partial results
 };
 
@@ -980,67 +981,109 @@ constexpr int walk_waves(int head_dim) { return head_dim == 256 ? 2 : 4; }  // o
 constexpr int walk_occ(int head_dim) { return head_dim == 256 ? 1 : 2; }
 constexpr int rows_occ(int head_dim, int nqt) { return head_dim == 256 || nqt > 1 ? 2 : 3; }
 
-// workspace_bytes: what partial results may take (the units are shared out over no more workgroups than fit).
-static WalkShape walk_shape(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, size_t workspace_bytes) {
+// What the kernels take, by the query rows of a group, in us at 128 dims: per unit of a workgroup that has a compute unit to itself
+// (alone), per unit and workgroup of a compute unit that is full, and for every further workgroup of a compute unit to start.  (Measured over 4-bit pools with 8 KV heads, 4 query heads each:
+// one sequence x 4096 tokens, 128 / 512 new ones, in groups of 16: 32 / 91 us, 64: 103 / 104, 128: 129 / 131; 4 sequences x 4608, 512
+// new ones: 355 / 247 / 190.)
+struct WalkKind {
+  int nqt, group_rows;  // nqt 0: walk_attn_kernel
+  double alone, full, start;
+};
+static WalkKind walk_kind(int kind, int head_dim) {
+  if (head_dim == 256) return kind == 0 ? WalkKind{0, 16, 0.75, 0.72, 1.8} : WalkKind{1, 64, 1.1, 0.65, 4.0};
+  const double f = 0.27 + 0.73 * head_dim / 128;
+  return kind == 0   ? WalkKind{0, 16, 0.165 * f, 0.165 * f, 1.8}
+         : kind == 1 ? WalkKind{1, 64, 0.77 * f, 0.43 * f, 4.0}
+                     : WalkKind{2, 128, 1.0 * f, 0.65 * f, 8.0};
+}
+
+// The shape of a launch in groups of one kind, and an estimate of its time in us.
+static WalkShape walk_shape_of(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, const WalkKind& kind, double& time) {
   WalkShape s = {};
-  const int64_t rows = a->q_len * (int64_t)(a->num_q_heads / pool->num_kv_heads);
+  const int64_t n_rep = a->num_q_heads / pool->num_kv_heads, rows = a->q_len * n_rep;
   const int D = pool->head_dim, heads = pool->num_kv_heads;
-  s.nqt = rows <= 16 ? 0 : (rows <= 64 || D == 256 ? 1 : 2);
-  s.group_rows = s.nqt == 0 ? 16 : 64 * s.nqt;
+  const bool few = kind.nqt == 0;
+  s.nqt = kind.nqt, s.group_rows = kind.group_rows;
   s.n_qgroups = (int)((rows + s.group_rows - 1) / s.group_rows);
   s.slot_rows = (int)std::min<int64_t>(rows, s.group_rows);
   int64_t units = ((int64_t)a->max_seq_len + 31) / 32;  // of the longest group
   if (a->window > 0) {
-    const int64_t n_rep = rows / std::max(a->q_len, 1), tokens = std::min<int64_t>(a->q_len, (s.slot_rows - 1) / std::max<int64_t>(n_rep, 1) + 2);
+    const int64_t tokens = std::min<int64_t>(a->q_len, (s.slot_rows - 1) / std::max<int64_t>(n_rep, 1) + 2);
     units = std::min(units, (a->window + (a->causal ? tokens : a->q_len)) / 32 + 2 + a->sinks / 32 + 2);
   }
-  units = std::max<int64_t>(units, 1);
-  s.min_share = s.nqt == 0 ? walk_waves(D) : 1;  // units a workgroup works on side by side
-  const int64_t n_groups = (int64_t)a->batch * s.n_qgroups, groups = n_groups * heads;
-  // Workgroups that run side by side and keep the GPU busy.  One per compute unit nearly is enough for walk_attn_kernel, whose
-  // waves fetch ahead; where its units are shared out it gets two (64 x 500 .. 8000 tokens: 71 us with one, 60 with two).
-  const int64_t slots = (int64_t)compute_units() * (s.nqt == 0 ? 1 : rows_occ(D, s.nqt));
+  s.units = units = std::max<int64_t>(units, 1);
+  s.min_share = few ? walk_waves(D) : 1;  // units a workgroup works on side by side
+  const int64_t n_groups = (int64_t)a->batch * s.n_qgroups, groups = n_groups * heads, cus = compute_units();
+  // One workgroup per compute unit nearly is enough for walk_attn_kernel, whose waves fetch ahead; where its units are shared out it
+  // gets two (64 x 500 .. 8000 tokens: 71 us with one, 60 with two).
+  const int64_t slots = cus * (few ? 2 : rows_occ(D, s.nqt));
   int64_t shares = 0;
   if (n_groups * units >= (int64_t)1 << 30) {
-    // (the run of all units is counted in 32 bits; as many groups as that need no sharing)
+    time = 1e30;  // (the run of all units is counted in 32 bits; as many groups as that need no sharing)
   } else if (a->partition_tokens > 0) {
+    time = 0;
     s.part_units = (a->partition_tokens / 32 + s.min_share - 1) / s.min_share * s.min_share;
     shares = n_groups == 1 ? (units + s.part_units - 1) / s.part_units : (n_groups * units + s.part_units - 1) / s.part_units;
     if (units <= s.part_units && n_groups == 1) shares = 0;
   } else {
-    // Sharing costs a second launch and a trip of the partial results.  It pays where a workgroup per group would leave much of the
-    // GPU idle: throughout, in its last round, or because some sequence may be far longer than the others (lengths are not
-    // known here, only their bound).  Measured without -> with, 8 KV heads of 128 dims, 4 query heads each, us:
-    //   one row, 1 x 4096 tokens: 28 -> 10.5; 33 x 8000: 99 -> 73; 64 x 500 .. 8000: 76 -> 60; 64 x 8000: 113 -> 127;
-    //     256 x 100 .. 8000: 154 -> 175; through a window of 4096, 32 sequences: 83 -> 91
+    // A workgroup per group lasts as long as the longest chain of units, or as a compute unit with its workgroups needs: under the causal
+    // limit the groups of a fresh prompt have half as many units on average.  Sequences of long contexts may differ in
+    // length (only the bound is known here), which leaves compute units idle, unless there are many.
+    const double average = a->causal && a->window == 0 ? (double)units * (1.0 - 0.5 * std::min(a->q_len, a->max_seq_len) / std::max(a->max_seq_len, 1)) : (double)units;
+    const double ragged = rows <= 128 && a->batch > 1 && units > 160 ? 1.4 : 1.0;
+    const int64_t per_cu = (groups + cus - 1) / cus;
+    const double own = (7.0 + std::max(units * kind.alone, average * kind.full * (double)per_cu) + kind.start * (double)(per_cu - 1)) * ragged;
+    // Equal shares of all units cost a second launch, the start of more pieces, and a trip of the partial results: some 10 us, 4 next to a
+    // single group, 12 to 40 where four waves work in step, and 10 more per 9216 rows.  Measured without -> with, 8 KV heads of 128 dims,
+    // 4 query heads each, us:
+    //   one row, 1 x 512 tokens: 8.6 -> 9.8; 1 x 4096: 28 -> 10.5; 8 x 2000: 17.7 -> 19.8; 33 x 8000: 99 -> 73;
+    //     64 x 500 .. 8000: 76 -> 60; 64 x 8000: 113 -> 127; 256 x 100 .. 8000: 154 -> 175; a window of 4096, 32 sequences: 83 -> 91
     //   9 drafted tokens, 32 x 1000 .. 6000: 146 -> 64; 96 x 500 .. 8000: 224 -> 148; 192 x 500 .. 8000: 350 -> 302; 192 x 6000: 535 -> 534
-    //   chunks of 512, 2 x 8000: 266 -> 223; 4 x 8000: 392 -> 425; 4 x 800 .. 8000: 269 -> 313; 9 x 8000: 774 -> 852
-    // so: where less than a round of workgroups is there, and, where each has a sequence of its own, up to the rounds after which
-    // unequal lengths even out by themselves.  Not for groups of few units: they end before a second launch does.
-    const double idle = (double)((groups + slots - 1) / slots * slots) / (double)groups;
-    const int64_t few = s.nqt == 0 ? 8 : 16;
-    const bool own_sequence = s.n_qgroups == 1 && groups <= slots * (s.nqt == 0 ? 4 : 2);
-    if (units > few && ((groups < slots && idle > 1.2) || (own_sequence && (units > 160 || idle > 1.2)))) {
-      shares = std::max<int64_t>((s.nqt == 0 ? 2 : 1) * slots / heads, 1);
-      if (s.nqt != 0) s.min_share = 4;
+    //   512 tokens, 2 x 8000: 266 -> 223; 4 x 8000: 392 -> 425; 4 x 800 .. 8000: 269 -> 313; a prompt of 1024: 39 -> 68
+    const double work = average * kind.full * (double)groups / (double)cus;
+    const double shared = 7.0 + 10.0 / 9216 * (double)(rows * a->batch * heads) + (few ? (n_groups == 1 ? 4.0 : 10.0) + work : std::max(40.0, 12.0 + work));
+    time = own;
+    if (shared < own && units > 8 && groups <= slots * 2) {
+      time = shared;
+      shares = std::max<int64_t>(slots / heads, 1);
+      if (!few) s.min_share = 4;
       if (n_groups == 1) {
-        s.part_units = (int)std::max<int64_t>((units + shares - 1) / shares, s.nqt == 0 ? 4 : 12);
+        s.part_units = (int)std::max<int64_t>((units + shares - 1) / shares, few ? 4 : 12);
         s.part_units = (s.part_units + s.min_share - 1) / s.min_share * s.min_share;
         shares = (units + s.part_units - 1) / s.part_units;
         if (shares == 1) shares = 0;
       }
     }
   }
-  const size_t one = (size_t)heads * 2 * s.slot_rows * (D + 2) * sizeof(float);  // of a workgroup per KV head
-  if (shares > 0 && workspace_bytes / one < (size_t)shares) {
-    shares = (int64_t)(workspace_bytes / one);
-    if (shares <= n_groups) shares = 0;  // (a workgroup per group does as well)
-    s.part_units = 0;
-    if (shares > 0 && n_groups == 1) s.part_units = (int)(((units + shares - 1) / shares + s.min_share - 1) / s.min_share * s.min_share);
-  }
   s.shares = (int)shares;
-  if (shares == 0) s.part_units = 0;
-  s.bytes = one * (size_t)shares;
+  return s;
+}
+
+// Groups of 16 rows (every wave unpacks for itself, four units of a group at a time) leave the shortest chain, groups of 128 the least
+// work: the estimates above decide, for a batch of short appends as for a long prompt.  Measured in groups of 16 / 64 / 128:
+// a prompt of 256 tokens 9.2 / 12.7 / 16.5 us, of 1024 40 / 31 / 39, 4 of 512 60 / 32 / 33; 9 tokens to 8 x 2000 19 / 35 / 40.
+// workspace_bytes: what partial results may take (the units are shared out over no more workgroups than fit).
+static WalkShape walk_shape(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, size_t workspace_bytes) {
+  const int64_t rows = a->q_len * (int64_t)(a->num_q_heads / pool->num_kv_heads);
+  const int D = pool->head_dim, heads = pool->num_kv_heads;
+  const int largest = rows <= 16 ? 0 : (rows <= 64 || D == 256 ? 1 : 2);
+  double best = 0;
+  WalkShape s = walk_shape_of(pool, a, walk_kind(largest, D), best);
+  for (int kind = largest - 1; kind >= 0; --kind) {  // (given partitions: the largest groups)
+    double time = 0;
+    const WalkShape t = walk_shape_of(pool, a, walk_kind(kind, D), time);
+    if (time < best) s = t, best = time;
+  }
+  const int64_t n_groups = (int64_t)a->batch * s.n_qgroups;
+  const size_t one = (size_t)heads * 2 * s.slot_rows * (D + 2) * sizeof(float);  // of a workgroup per KV head
+  if (s.shares > 0 && workspace_bytes / one < (size_t)s.shares) {
+    s.shares = (int)(workspace_bytes / one);
+    if (s.shares <= n_groups) s.shares = 0;  // (a workgroup per group does as well)
+    s.part_units = 0;
+    if (s.shares > 0 && n_groups == 1) s.part_units = (int)(((s.units + s.shares - 1) / s.shares + s.min_share - 1) / s.min_share * s.min_share);
+  }
+  if (s.shares == 0) s.part_units = 0;
+  s.bytes = one * (size_t)s.shares;
   return s;
 }
 

@@ -100,7 +100,7 @@ def test_workspaces_of_any_size(device, S):
     table, lens_dev = c.state.device_table(), torch.tensor(lens, dtype=torch.int32, device=device)
     a = nat.PagedAttnArgs(q=qd.data_ptr(), q_stride_b=qd.stride(0), q_stride_h=qd.stride(1), q_stride_s=qd.stride(2), block_table=table.data_ptr(),
                           table_stride=table.stride(0), seq_lens=lens_dev.data_ptr(), batch=4, num_q_heads=H * rep, q_len=S, causal=1,
-                          max_seq_len=3000, scale=1 / math.sqrt(D))
+                          max_seq_len=3000, partition_tokens=256, scale=1 / math.sqrt(D))  # (cut whether that pays or not)
     need = int(lib.pace_paged_attn_workspace_for(ctypes.byref(c.pool_desc), ctypes.byref(a)))
     assert need > 0
     for size in (0, 1000, need // 50, need // 7, need // 2, need - 1, need, need + 4096):
