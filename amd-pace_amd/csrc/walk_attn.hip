@@ -875,96 +875,105 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
 }
 
 // out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the partial results of a query row.  A wave takes eight at a time, a lane the
-// dims 2 lane, 2 lane + 1 (+ 128); WPR waves share a row (partial results in turn, joined through LDS).  Rows of groups that
+// dims 2 lane, 2 lane + 1 (+ 128); WPR waves share a row (partial results in turn, joined through LDS), or a wave takes
+// ROWS rows after one look at the lengths.  Rows of groups that
 // one workgroup covered are finished already; rows that read nothing belong to no workgroup and become 0 here.
 // Bound: latency (a launch, the lengths, then the partial results): some 5 us next to one sequence, up to 10 next to 9216 rows.
-template <int D, int WPR>
+template <int D, int WPR, int ROWS>
 __global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int32_t total_rows) {
   constexpr int PASSES = (D + 127) / 128;
   __shared__ float join[WPR > 1 ? WPR : 1][2 * PASSES + 2][WPR > 1 ? 64 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave % WPR;
-  const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;  // (b, hq, s)
-  if (row >= total_rows) return;  // (WPR == 1 only: whole waves; else the grid is exact)
-  const int S = p.q_len, s = (int)(row % S), hq = (int)(row / S % p.num_q_heads), b = (int)(row / S / p.num_q_heads);
-  const int kvh = hq / p.n_rep, r = s * p.n_rep + hq % p.n_rep, qg = r / p.group_rows;
-  const int j = b * p.n_qgroups + p.n_qgroups - 1 - qg;
-  int units, share, at;  // of the row's group: units, and where they begin in the run of all units
-  if (p.part_units > 0 && p.batch * p.n_qgroups == 1) {
-    units = group_units(p, 0), share = p.part_units, at = 0;
+  const int64_t row0 = WPR > 1 ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * 4 + wave) * ROWS;  // (b, hq, s)
+  if (row0 >= total_rows) return;  // (WPR == 1 only: whole waves)
+  const int S = p.q_len, n_groups = p.batch * p.n_qgroups;
+  const bool one_group = p.part_units > 0 && n_groups == 1;
+  int mine, share;  // units of the first 64 groups, one per lane
+  if (one_group) {
+    mine = group_units(p, 0), share = p.part_units;
   } else {
-    int before = 0, total = 0;
+    mine = group_units(p, lane);
+    int total = mine;
 #pragma unroll 4
-    for (int i = lane; i < p.batch * p.n_qgroups; i += 64) {
-      const int u = group_units(p, i);
-      total += u, before += i < j ? u : 0;
-    }
-    total = wave_sum(total), at = wave_sum(before);
-    share = walk_share(p, total);
-    units = group_units(p, j);
+    for (int i = lane + 64; i < n_groups; i += 64) total += group_units(p, i);
+    share = walk_share(p, wave_sum(total));
   }
-  const int w0 = at / share, n_parts = units > 0 ? min((at + units - 1) / share, p.shares - 1) - w0 + 1 : 0;
-  if (n_parts == 1) return;  // uniform over the row's waves
-  // workgroup w0 + i's piece lies in its first slot, except the first one's if that workgroup began with other groups
-  const int late = at % share != 0 ? 1 : 0;
-  auto place = [&](int i) { return ((int64_t)(2 * (w0 + i) + (i == 0 ? late : 0)) * p.num_kv_heads + kvh) * p.slot_rows + (r - qg * p.group_rows); };
-  const int d0 = 2 * lane;
-  float acc[PASSES][2], M = kNegInf, L = 0.f;
-#pragma unroll
-  for (int e = 0; e < PASSES; ++e) acc[e][0] = acc[e][1] = 0.f;
-  for (int base = 8 * slice; base < n_parts; base += 8 * WPR) {
-    const u32x2 pair = *reinterpret_cast<const u32x2*>(p.part_ml + 2 * place(min(base + (lane & 7), n_parts - 1)));
-    u32x2 v[8][PASSES];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < PASSES; ++e) {
-        v[i][e] = u32x2{0u, 0u};
-        if (base + i < n_parts && d0 + 128 * e < D) v[i][e] = *reinterpret_cast<const u32x2*>(p.part_o + place(base + i) * D + d0 + 128 * e);
-      }
-    const float m_mine = base + (lane & 7) < n_parts ? __uint_as_float(pair[0]) : kNegInf;
-    float top = m_mine;
-    top = fmaxf(top, __shfl_xor(top, 1, 64)), top = fmaxf(top, __shfl_xor(top, 2, 64)), top = fmaxf(top, __shfl_xor(top, 4, 64));
-    const float M_new = fmaxf(M, top), m_use = M_new == kNegInf ? 0.f : M_new, old = __builtin_amdgcn_exp2f(M - m_use);
-    const float w_mine = __builtin_amdgcn_exp2f(m_mine - m_use);
-    M = M_new, L *= old;
-#pragma unroll
-    for (int e = 0; e < PASSES; ++e) acc[e][0] *= old, acc[e][1] *= old;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (base + i < n_parts) {  // wave-uniform
-        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_mine), i));
-        L += w * __uint_as_float(__builtin_amdgcn_readlane(pair[1], i));
-#pragma unroll
-        for (int e = 0; e < PASSES; ++e) acc[e][0] += w * __uint_as_float(v[i][e][0]), acc[e][1] += w * __uint_as_float(v[i][e][1]);
-      }
+  int last_j = -1, w0 = 0, n_parts = 0, late = 0;
+  for (int64_t row = row0; row < row0 + ROWS && row < total_rows; ++row) {
+    const int s = (int)(row % S), hq = (int)(row / S % p.num_q_heads), b = (int)(row / S / p.num_q_heads);
+    const int kvh = hq / p.n_rep, r = s * p.n_rep + hq % p.n_rep, qg = r / p.group_rows;
+    const int j = b * p.n_qgroups + p.n_qgroups - 1 - qg;
+    if (j != last_j) {  // the group's units, and where they begin in the run of all units
+      int before = lane < j ? mine : 0;
+      for (int i = lane + 64; i < j; i += 64) before += group_units(p, i);
+      const int at = one_group ? 0 : wave_sum(before);
+      const int units = j < 64 ? __builtin_amdgcn_readlane(mine, j) : group_units(p, j);
+      w0 = at / share, n_parts = units > 0 ? min((at + units - 1) / share, p.shares - 1) - w0 + 1 : 0;
+      late = at % share != 0 ? 1 : 0;
+      last_j = j;
     }
-  }
-  if constexpr (WPR > 1) {
-#pragma unroll
-    for (int e = 0; e < PASSES; ++e) join[slice][2 * e][lane] = acc[e][0], join[slice][2 * e + 1][lane] = acc[e][1];
-    join[slice][2 * PASSES][lane] = M, join[slice][2 * PASSES + 1][lane] = L;
-    __syncthreads();
-    if (slice != 0) return;
-    float all = kNegInf;
-#pragma unroll
-    for (int w = 0; w < WPR; ++w) all = fmaxf(all, join[w][2 * PASSES][lane]);
-    const float m_use = all == kNegInf ? 0.f : all;
-    L = 0.f;
+    if (n_parts == 1) continue;  // uniform over the row's waves
+    // workgroup w0 + i's piece lies in its first slot, except the first one's if that workgroup began with other groups
+    auto place = [&](int i) { return ((int64_t)(2 * (w0 + i) + (i == 0 ? late : 0)) * p.num_kv_heads + kvh) * p.slot_rows + (r - qg * p.group_rows); };
+    const int d0 = 2 * lane;
+    float acc[PASSES][2], M = kNegInf, L = 0.f;
 #pragma unroll
     for (int e = 0; e < PASSES; ++e) acc[e][0] = acc[e][1] = 0.f;
+    for (int base = 8 * slice; base < n_parts; base += 8 * WPR) {
+      const u32x2 pair = *reinterpret_cast<const u32x2*>(p.part_ml + 2 * place(min(base + (lane & 7), n_parts - 1)));
+      u32x2 v[8][PASSES];
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) {
-      const float f = __builtin_amdgcn_exp2f(join[w][2 * PASSES][lane] - m_use);
-      L += f * join[w][2 * PASSES + 1][lane];
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int e = 0; e < PASSES; ++e) acc[e][0] += f * join[w][2 * e][lane], acc[e][1] += f * join[w][2 * e + 1][lane];
+        for (int e = 0; e < PASSES; ++e) {
+          v[i][e] = u32x2{0u, 0u};
+          if (base + i < n_parts && d0 + 128 * e < D) v[i][e] = *reinterpret_cast<const u32x2*>(p.part_o + place(base + i) * D + d0 + 128 * e);
+        }
+      const float m_mine = base + (lane & 7) < n_parts ? __uint_as_float(pair[0]) : kNegInf;
+      float top = m_mine;
+      top = fmaxf(top, __shfl_xor(top, 1, 64)), top = fmaxf(top, __shfl_xor(top, 2, 64)), top = fmaxf(top, __shfl_xor(top, 4, 64));
+      const float M_new = fmaxf(M, top), m_use = M_new == kNegInf ? 0.f : M_new, old = __builtin_amdgcn_exp2f(M - m_use);
+      const float w_mine = __builtin_amdgcn_exp2f(m_mine - m_use);
+      M = M_new, L *= old;
+#pragma unroll
+      for (int e = 0; e < PASSES; ++e) acc[e][0] *= old, acc[e][1] *= old;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (base + i < n_parts) {  // wave-uniform
+          const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_mine), i));
+          L += w * __uint_as_float(__builtin_amdgcn_readlane(pair[1], i));
+#pragma unroll
+          for (int e = 0; e < PASSES; ++e) acc[e][0] += w * __uint_as_float(v[i][e][0]), acc[e][1] += w * __uint_as_float(v[i][e][1]);
+        }
+      }
     }
-  }
-  const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
-  uint16_t* op = p.out + (int64_t)b * p.o_sb + (int64_t)hq * p.o_sh + (int64_t)s * p.o_ss + d0;
+    if constexpr (WPR > 1) {
 #pragma unroll
-  for (int e = 0; e < PASSES; ++e)
-    if (d0 + 128 * e < D) *reinterpret_cast<uint32_t*>(op + 128 * e) = pack_bf16x2(acc[e][0] * inv, acc[e][1] * inv);
+      for (int e = 0; e < PASSES; ++e) join[slice][2 * e][lane] = acc[e][0], join[slice][2 * e + 1][lane] = acc[e][1];
+      join[slice][2 * PASSES][lane] = M, join[slice][2 * PASSES + 1][lane] = L;
+      __syncthreads();
+      if (slice != 0) continue;
+      float all = kNegInf;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) all = fmaxf(all, join[w][2 * PASSES][lane]);
+      const float m_use = all == kNegInf ? 0.f : all;
+      L = 0.f;
+#pragma unroll
+      for (int e = 0; e < PASSES; ++e) acc[e][0] = acc[e][1] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) {
+        const float f = __builtin_amdgcn_exp2f(join[w][2 * PASSES][lane] - m_use);
+        L += f * join[w][2 * PASSES + 1][lane];
+#pragma unroll
+        for (int e = 0; e < PASSES; ++e) acc[e][0] += f * join[w][2 * e][lane], acc[e][1] += f * join[w][2 * e + 1][lane];
+      }
+    }
+    const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+    uint16_t* op = p.out + (int64_t)b * p.o_sb + (int64_t)hq * p.o_sh + (int64_t)s * p.o_ss + d0;
+#pragma unroll
+    for (int e = 0; e < PASSES; ++e)
+      if (d0 + 128 * e < D) *reinterpret_cast<uint32_t*>(op + 128 * e) = pack_bf16x2(acc[e][0] * inv, acc[e][1] * inv);
+  }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
@@ -1149,11 +1158,13 @@ int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, con
     } else {
       if (masked) launch_walk_kernel<16, D, true>(p, sh.nqt, stream); else launch_walk_kernel<16, D, false>(p, sh.nqt, stream);
     }
-    // few groups, many workgroups each: four waves to a row
-    if (sh.shares > 4 * (int64_t)a->batch * sh.n_qgroups)
-      hipLaunchKernelGGL((walk_merge_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, p, (int32_t)rows);
-    else if (sh.shares > 0)
-      hipLaunchKernelGGL((walk_merge_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p, (int32_t)rows);
+    // Few groups, many workgroups each: four waves to a row.  More rows than the GPU holds waves: four rows to a wave, one look at the
+    // lengths for all (with the attention, one row -> four: 512 tokens to 4096 83 -> 79 us, 9 to 96 x 500 .. 8000 148 -> 143).
+    const bool wide = sh.shares > 4 * (int64_t)a->batch * sh.n_qgroups, many = rows >= (size_t)compute_units() * 32;
+    if (sh.shares == 0) return;
+    if (wide) hipLaunchKernelGGL((walk_merge_kernel<D, 4, 1>), dim3((unsigned)rows), dim3(256), 0, stream, p, (int32_t)rows);
+    else if (many) hipLaunchKernelGGL((walk_merge_kernel<D, 1, 4>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, p, (int32_t)rows);
+    else hipLaunchKernelGGL((walk_merge_kernel<D, 1, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p, (int32_t)rows);
   });
   PACE_HIP_CHECK(hipGetLastError());
   return PACE_KV_OK;
