@@ -26,9 +26,9 @@ struct WalkParams : PagedAttnParams {
   int32_t slot_rows;      // query rows of a partial result
   // How the groups (sequence, run of query rows) are dealt to workgroups.  shares == 0: one workgroup per group and KV head.  Else
   // the units of all groups of a KV head lie end to end and `shares` workgroups take equal runs of them (at least
-  // min_share and part_units), so that a batch of any lengths keeps every workgroup busy for the same time.  A group that one workgroup covers alone is finished there; pieces of others
-  // become partial results, two per workgroup at most -- the group it starts in the middle of or with, and the one it
-  // breaks off -- which walk_merge_kernel joins.
+  // min_share and part_units), so that a batch of any lengths keeps every workgroup busy for the same time.  A group that one
+  // workgroup covers alone is finished there; pieces of others become partial results, two per workgroup at most -- the
+  // group it starts in the middle of or with, and the one it breaks off -- which walk_merge_kernel joins.
   int32_t shares, min_share, part_units;
 };
 
@@ -587,8 +587,8 @@ struct WalkTurns {
 };
 
 // ---------------------------------------------------------------------------------
-// Groups of up to 16 query rows (decode; short appends, and prompts too short to fill the GPU otherwise): every wave walks units of its own.  NW waves split a workgroup's units (wave w:
-// units w, w + NW, ...), fetch one ahead, and merge through LDS.
+// Groups of up to 16 query rows (decode; short appends, and prompts too short to fill the GPU otherwise): every wave walks units of
+// its own.  NW waves split a workgroup's units (wave w: units w, w + NW, ...), fetch one ahead, and merge through LDS.
 //
 // Bound: the pool's bytes.  64 sequences x 4096 tokens, 8 KV heads of 128 dims, 4 query heads each: 57 us for 336 MB of
 // 4-bit rows, 5.9 TB/s, where a plain read of as much reaches 6.0; 32 sequences through a window of 4096 tokens over a bf16
@@ -991,9 +991,9 @@ constexpr int walk_occ(int head_dim) { return head_dim == 256 ? 1 : 2; }
 constexpr int rows_occ(int head_dim, int nqt) { return head_dim == 256 || nqt > 1 ? 2 : 3; }
 
 // What the kernels take, by the query rows of a group, in us at 128 dims: per unit of a workgroup that has a compute unit to itself
-// (alone), per unit and workgroup of a compute unit that is full, and for every further workgroup of a compute unit to start.  (Measured over 4-bit pools with 8 KV heads, 4 query heads each:
-// one sequence x 4096 tokens, 128 / 512 new ones, in groups of 16: 32 / 91 us, 64: 103 / 104, 128: 129 / 131; 4 sequences x 4608, 512
-// new ones: 355 / 247 / 190.)
+// (alone), per unit and workgroup of a compute unit that is full, and for every further workgroup of a compute unit to start.
+// (Measured over 4-bit pools with 8 KV heads, 4 query heads each: one sequence x 4096 tokens, 128 / 512 new ones, in groups
+// of 16: 32 / 91 us, 64: 103 / 104, 128: 129 / 131; 4 sequences x 4608, 512 new ones: 355 / 247 / 190; 64 dims take 0.63 of it.)
 struct WalkKind {
   int nqt, group_rows;  // nqt 0: walk_attn_kernel
   double alone, full, start;
@@ -1038,7 +1038,8 @@ static WalkShape walk_shape_of(const pace_kv_pool_t* pool, const pace_paged_attn
     // A workgroup per group lasts as long as the longest chain of units, or as a compute unit with its workgroups needs: under the causal
     // limit the groups of a fresh prompt have half as many units on average.  Sequences of long contexts may differ in
     // length (only the bound is known here), which leaves compute units idle, unless there are many.
-    const double average = a->causal && a->window == 0 ? (double)units * (1.0 - 0.5 * std::min(a->q_len, a->max_seq_len) / std::max(a->max_seq_len, 1)) : (double)units;
+    const double fresh = a->causal && a->window == 0 ? std::min(a->q_len, a->max_seq_len) / (double)std::max(a->max_seq_len, 1) : 0.0;
+    const double average = (double)units * (1.0 - 0.5 * fresh);
     const double ragged = rows <= 128 && a->batch > 1 && units > 160 ? 1.4 : 1.0;
     const int64_t per_cu = (groups + cus - 1) / cus;
     const double own = (7.0 + std::max(units * kind.alone, average * kind.full * (double)per_cu) + kind.start * (double)(per_cu - 1)) * ragged;
