@@ -358,7 +358,8 @@ class PagedKVCache(KVCacheBase):
                     self._query_rope = None
             else:
                 self._pending = (k, v, head_step, rope)
-                self._query_rope = rope
+                if not keep_query_rope:
+                    self._query_rope = rope
             self.lens = self.lens + T
             self.seq_len += T
             return
