@@ -1098,6 +1098,7 @@ static WalkShape walk_shape(const pace_kv_pool_t* pool, const pace_paged_attn_ar
 }
 
 size_t walk_workspace_bytes(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a) {
+  if (a->partition_tokens < 0 || a->partition_tokens % 32 != 0) return 0;  // (the launch refuses it)
   return walk_shape(pool, a, ~(size_t)0).bytes;
 }
 

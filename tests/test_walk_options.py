@@ -1,0 +1,30 @@
+"""Options of the 4-bit cache and of the window, and sizes a launch is asked about, that need no GPU."""
+import ctypes
+import os
+import subprocess
+import sys
+
+from test_q4_oracle import _args, _pool
+
+
+def need(elem_bytes=1, **kw):
+    """The scratch the library asks for."""
+    from pace_mi355 import _native as nat
+
+    pool = _pool(nat) if elem_bytes == 1 else _pool(nat, elem_bytes=elem_bytes, k_block_stride=1 << 17, k_head_stride=1 << 13,
+                                                    v_block_stride=1 << 17, v_head_stride=1 << 13)
+    return int(nat.load().pace_paged_attn_workspace_for(ctypes.byref(pool), ctypes.byref(_args(nat, **kw))))
+
+
+def test_a_cut_that_is_no_multiple_of_32_needs_nothing():
+    """(In a process of its own, which a division by zero would end.)"""
+    code = ("from test_walk_options import need\n"
+            "for elem, window in ((1, 0), (2, 64)):\n"
+            "  for tokens in (1, 16, 31, 33, 48, -1, -32):\n"
+            "    for batch, q_len in ((1, 1), (8, 1), (1, 9), (3, 100)):\n"
+            "      got = need(elem, batch=batch, q_len=q_len, max_seq_len=4096, partition_tokens=tokens, window=window)\n"
+            "      assert got == 0, (elem, tokens, batch, q_len, got)\n"
+            "print('done')")
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(p for p in sys.path if p))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, env=env, cwd=os.path.dirname(os.path.abspath(__file__)))
+    assert r.returncode == 0 and r.stdout.split() == ["done"], f"exit status {r.returncode}: {r.stderr[-500:]}"
