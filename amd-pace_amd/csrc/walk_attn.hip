@@ -651,6 +651,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     min_limit = __builtin_amdgcn_readfirstlane(min_limit);
     const int row_low = p.window > 0 ? len - S + x.s_first - p.window + 1 : 0;  // the first row's window, and the last row's
     const int max_low = p.window > 0 ? len - S + x.s_last - p.window + 1 : 0;
+    const int row_end = p.causal ? min(len, len - S + x.s_last + 1) : len;
 
     auto take = [&](WalkUnit<BITS, D>& u, const MaskRaw<1>& m, int k) {
       const int t0 = 32 * walk.unit(i_begin + wave + NW * k);
@@ -660,7 +661,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
         if (walk_masked_out<D, 1>(mregs, st)) return;
       }
       const bool full = t0 >= start && t0 + 31 <= min_limit && (t0 >= max_low || t0 + 32 <= walk.sink_end);
-      if (BITS == 16 && !full) u.drop(walk_keep(t0, g, start, walk.sink_end, row_low, len));
+      if (BITS == 16 && !full) u.drop(walk_keep(t0, g, start, walk.sink_end, row_low, row_end));
       f32x4 sc[1][2];
       u32x4 pb[1];
       walk_scores<BITS, D, 1, 1>([&](int t, int kk) { return u.k(t, kk); }, st, sc);
