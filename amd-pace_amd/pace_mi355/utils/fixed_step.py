@@ -81,7 +81,13 @@ class FixedStep:
         a.batch, a.num_q_heads, a.q_len = B, hq, S
         # the library's planner cuts the batch: descriptors of (sequence, partition) work items in scheduling order
         a.max_seq_len, a.partition_tokens, a.scale = max_len, 0, 1.0 / math.sqrt(D)
-        if cache.f32:  # rows of fp32: one launch over the block table, no work list; the workspace lets a small batch be cut
+        walk = cache.kv_bits == 4 or cache.window > 0  # kernels that need no work list
+        a.window, a.sinks = cache.window, cache.sinks
+        if walk:
+            a.partition_tokens = partition
+            n_items = max_parts = 0
+            ws_bytes = int(self.lib.pace_paged_attn_workspace_for(ctypes.byref(cache._desc), ctypes.byref(a)))
+        elif cache.f32:  # rows of fp32: one launch over the block table, no work list; the workspace lets a small batch be cut
             n_items = max_parts = 0
             ws_bytes = min(B * hq * S * 64 * (D + 4) * 4, 64 << 20)
         else:
