@@ -26,7 +26,8 @@ struct WalkParams : PagedAttnParams {
   int32_t slot_rows;      // query rows of a partial result
   // How the groups (sequence, run of query rows) are dealt to workgroups.  shares == 0: one workgroup per group and KV head.  Else
   // the units of all groups of a KV head lie end to end and `shares` workgroups take equal runs of them (at least
-  // min_share and part_units), so that a batch of any lengths keeps every workgroup busy for the same time.  A group that one
+  // min_share), so that a batch of any lengths keeps every workgroup busy for the same time; the units of a single group
+  // are dealt out part_units at a time, which asks for no sum over lengths.  A group that one
   // workgroup covers alone is finished there; pieces of others become partial results, two per workgroup at most -- the
   // group it starts in the middle of or with, and the one it breaks off -- which walk_merge_kernel joins.
   int32_t shares, min_share, part_units;
@@ -83,7 +84,7 @@ struct Shares {
   int total, share;
 };
 __device__ __forceinline__ int walk_share(const WalkParams& p, int total) {
-  return max(max((total + p.shares - 1) / p.shares, p.min_share), p.part_units);  // (unrounded: equal sequences stay whole)
+  return max((total + p.shares - 1) / p.shares, p.min_share);  // (unrounded: equal sequences stay whole)
 }
 __device__ __forceinline__ int wave_sum(int v) {
 #pragma unroll
@@ -1043,9 +1044,12 @@ static WalkShape walk_shape_of(const pace_kv_pool_t* pool, const pace_paged_attn
     time = 1e30;  // (the run of all units is counted in 32 bits; as many groups as that need no sharing)
   } else if (a->partition_tokens > 0) {
     time = 0;
-    s.part_units = (a->partition_tokens / 32 + s.min_share - 1) / s.min_share * s.min_share;
-    shares = n_groups == 1 ? (units + s.part_units - 1) / s.part_units : (n_groups * units + s.part_units - 1) / s.part_units;
-    if (units <= s.part_units && n_groups == 1) shares = 0;
+    // A given cut: no run is longer, and nothing is cut if no group is longer.  (The runs of several groups are equal shares here
+    // too, so sequences below max_seq_len make them shorter, not fewer.)
+    s.part_units = (int)(((int64_t)a->partition_tokens / 32 + s.min_share - 1) / s.min_share * s.min_share);
+    if (units > s.part_units) shares = (n_groups * units + s.part_units - 1) / s.part_units;  // (more than there are groups)
+    if (!few) s.min_share = std::min(s.part_units, 4);
+    if (n_groups > 1) s.part_units = 0;
   } else {
     // A workgroup per group lasts as long as the longest chain of units, or as a compute unit with its workgroups needs: under the causal
     // limit the groups of a fresh prompt have half as many units on average.  Sequences of long contexts may differ in

@@ -325,7 +325,9 @@ typedef struct pace_paged_attn_args {
   int32_t batch, num_q_heads, q_len;
   int32_t causal;             /* 1: query row s reads tokens <= seq_len - q_len + s    */
   int32_t max_seq_len;        /* host-side upper bound of seq_lens (sizes the grid)    */
-  int32_t partition_tokens;   /* context split size per workgroup, multiple of 32; 0 = auto   */
+  int32_t partition_tokens;   /* context split size per workgroup, multiple of 32; 0 = auto.  Over a 4-bit pool or through
+                                 a window: the most tokens a workgroup takes (in steps of 32 to 128, rounded up); what
+                                 no sequence exceeds cuts nothing */
   float scale;                /* softmax scale (> 0), reference uses 1/sqrt(head_dim)  */
   void* workspace;            /* device scratch, >= pace_paged_attn_workspace_bytes()  */
   size_t workspace_bytes;

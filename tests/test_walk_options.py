@@ -28,3 +28,14 @@ def test_a_cut_that_is_no_multiple_of_32_needs_nothing():
     env = dict(os.environ, PYTHONPATH=os.pathsep.join(p for p in sys.path if p))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, env=env, cwd=os.path.dirname(os.path.abspath(__file__)))
     assert r.returncode == 0 and r.stdout.split() == ["done"], f"exit status {r.returncode}: {r.stderr[-500:]}"
+
+
+def test_a_cut_is_the_longest_run_of_a_workgroup():
+    """Nothing is cut that fits, however many sequences there are, and no workgroup takes the sequences of others besides."""
+    piece = 8 * 2 * 4 * 130 * 4  # two partial results of 4 query rows for each of 8 KV heads: 128 dims, a maximum and a sum
+    for batch in (1, 2, 64):
+        for longest in (1, 100, 4096):
+            assert need(batch=batch, max_seq_len=longest, partition_tokens=4096) == 0, (batch, longest)
+        assert need(batch=batch, max_seq_len=8192, partition_tokens=4096) == 2 * batch * piece
+        assert need(batch=batch, max_seq_len=8192, partition_tokens=1 << 20) == 0
+        assert need(2, batch=batch, max_seq_len=1 << 17, partition_tokens=4096, window=2048, sinks=4) == 0  # the window fits
