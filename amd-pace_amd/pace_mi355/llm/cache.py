@@ -731,6 +731,8 @@ class KVCacheManager:
             ]
             shared["layers"] = self.cache_objects
         else:
+            if paged_options.get("kv_bits", 16) != 16 or paged_options.get("window") or paged_options.get("sinks"):
+                raise ValueError(f"kv_bits=4, window and sinks are options of the paged cache; got cache type {cache_type}")
             self.cache_objects = [self.kv_cache_class(max_seq_length) for _ in range(self.num_layers)]
 
     def __len__(self) -> int:

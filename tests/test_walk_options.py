@@ -4,6 +4,8 @@ import os
 import subprocess
 import sys
 
+import pytest
+
 from test_q4_oracle import _args, _pool
 
 
@@ -39,3 +41,20 @@ def test_a_cut_is_the_longest_run_of_a_workgroup():
         assert need(batch=batch, max_seq_len=8192, partition_tokens=4096) == 2 * batch * piece
         assert need(batch=batch, max_seq_len=8192, partition_tokens=1 << 20) == 0
         assert need(2, batch=batch, max_seq_len=1 << 17, partition_tokens=4096, window=2048, sinks=4) == 0  # the window fits
+
+
+class _Cfg:
+    num_hidden_layers = 2
+    num_attention_heads = 8
+    num_key_value_heads = 2
+
+
+@pytest.mark.parametrize("cache_type", ["dynamic", "bmc"])
+@pytest.mark.parametrize("option", [dict(kv_bits=4), dict(window=16), dict(window=16, sinks=2)])
+def test_caches_that_store_no_blocks_refuse_these_options(cache_type, option):
+    """They keep the model's dtype and their attention reads everything: taken silently, the options would change nothing."""
+    from pace_mi355.llm import KVCacheManager
+
+    with pytest.raises(ValueError, match="paged cache"):
+        KVCacheManager(_Cfg(), 64, cache_type, **option)
+    assert len(KVCacheManager(_Cfg(), 64, cache_type, kv_bits=16, window=None, sinks=0, num_blocks=8).cache_objects) == 2
