@@ -190,7 +190,7 @@ class PagedKVCache(KVCacheBase):
             raise RuntimeError("a window over an fp32 pool is not supported")
         if getattr(self, "pool", None) is not None:
             self._flush()  # a held-back append or a captured step belongs to the window it was made for
-        self.window, self.sinks = window, int(sinks)
+        self.window, self.sinks = (min(n, 2**31 - 1) for n in (window, int(sinks)))  # (the launch takes 32 bits, and so do positions)
 
     @property
     def pool_desc(self) -> Optional[nat.PoolDesc]:

@@ -58,3 +58,14 @@ def test_caches_that_store_no_blocks_refuse_these_options(cache_type, option):
     with pytest.raises(ValueError, match="paged cache"):
         KVCacheManager(_Cfg(), 64, cache_type, **option)
     assert len(KVCacheManager(_Cfg(), 64, cache_type, kv_bits=16, window=None, sinks=0, num_blocks=8).cache_objects) == 2
+
+
+@pytest.mark.parametrize("huge", [1 << 31, (1 << 32) + 5, 1 << 40])
+def test_a_window_wider_than_any_sequence_stays_one(huge):
+    """Positions are 32-bit numbers; a window or a count of sinks past them must not wrap around to a small one."""
+    from pace_mi355 import _native as nat
+    from pace_mi355.llm import PagedKVCache
+
+    c = PagedKVCache(64, window=huge, sinks=huge)
+    a = nat.PagedAttnArgs(window=c.window, sinks=c.sinks)
+    assert a.window == a.sinks == (1 << 31) - 1
