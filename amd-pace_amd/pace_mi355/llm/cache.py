@@ -583,6 +583,12 @@ class PagedKVCache(KVCacheBase):
         B, hq, S, D = query.shape
         if B != self.batch or D != self.model_dim or hq % self.num_kv_heads:
             raise RuntimeError(f"query {tuple(query.shape)} does not fit cache [B={self.batch}, Hkv={self.num_kv_heads}, D={self.model_dim}]")
+        if attention_mask is not None:
+            m = attention_mask
+            if m.dim() != 4 or m.size(1) != 1 or m.size(0) not in (1, B) or m.size(2) not in (1, S):
+                raise RuntimeError(f"paged attention takes a mask [B|1, 1, S|1, L]; got {tuple(m.shape)}")
+            if m.dtype not in (torch.float32, torch.bfloat16):
+                raise RuntimeError("pace::SDPA attention only support the dtypes Float and BF16 types for input Attention mask")
         if self.head_dim != self.model_dim:
             query, D = torch.nn.functional.pad(query, (0, self.head_dim - self.model_dim)), self.head_dim
         qs = query.stride()
@@ -592,7 +598,7 @@ class PagedKVCache(KVCacheBase):
             qs = query.stride()
         if self.f32 and self._pending is not None and self._graph is None and S * (hq // self.num_kv_heads) > 32:
             self._flush()  # over an fp32 pool the append rides in launches of up to 32 query rows per KV head
-        rope, self._query_rope = self._query_rope, None
+        rope = self._query_rope  # (a call that is refused leaves it, and a held-back append, for the next one)
         rope_desc = None
         if rope is not None:
             if tuple(rope.rows.shape) not in ((B, S), (1, S)):
@@ -667,10 +673,6 @@ class PagedKVCache(KVCacheBase):
         a.kv_start = None if kv_start is None else kv_start.data_ptr()
         if attention_mask is not None:
             m = attention_mask
-            if m.dim() != 4 or m.size(1) != 1 or m.size(0) not in (1, B) or m.size(2) not in (1, S):
-                raise RuntimeError(f"paged attention takes a mask [B|1, 1, S|1, L]; got {tuple(m.shape)}")
-            if m.dtype not in (torch.float32, torch.bfloat16):
-                raise RuntimeError("pace::SDPA attention only support the dtypes Float and BF16 types for input Attention mask")
             if m.stride(3) != 1:
                 m = m.contiguous()
             a.mask = m.data_ptr()
@@ -698,12 +700,12 @@ class PagedKVCache(KVCacheBase):
             k, v, head_step, k_rope = self._pending
             if (k_rope is None) != (rope_desc is None) or k.shape[2] != S and rope_desc is not None:
                 raise RuntimeError("a held-back append and the attention call disagree about the rotary embedding")
-            self._pending = None  # this launch stores them into the pool
             ks = k.stride()
             a.k_new, a.v_new, a.n_new = k.data_ptr(), v.data_ptr(), k.shape[2]
             a.new_stride_b, a.new_stride_h, a.new_stride_t = ks[0], ks[1] * head_step, ks[2]
         fn = lib.pace_paged_attn_decode if S == 1 else lib.pace_paged_attn_verify
         nat.check(fn(ctypes.byref(self._desc), ctypes.byref(a), nat.current_stream_ptr()))
+        self._query_rope = self._pending = None  # the launch stores a held-back append into the pool
         return out if self.head_dim == self.model_dim else out[..., : self.model_dim].contiguous()
 
 
