@@ -317,6 +317,8 @@ class PagedKVCache(KVCacheBase):
             raise RuntimeError(f"update of shape {tuple(k.shape)} does not fit cache [B={self.batch}, Hkv={self.num_kv_heads}, D={D}]")
         if v.shape != k.shape:
             raise RuntimeError("key_states and value_states differ in shape")
+        if k.device != self.pool.device or v.device != self.pool.device:
+            raise RuntimeError(f"the cache lies on {self.pool.device}; got key/value states on {k.device} / {v.device}")
         if self.head_dim != self.model_dim:
             # (a rotary embedding then rotates the first rotary_dim <= model_dim dims of the padded rows, in a launch of
             # its own: inside the attention launch it needs rotary_dim == the pool's head size)
@@ -583,8 +585,16 @@ class PagedKVCache(KVCacheBase):
         B, hq, S, D = query.shape
         if B != self.batch or D != self.model_dim or hq % self.num_kv_heads:
             raise RuntimeError(f"query {tuple(query.shape)} does not fit cache [B={self.batch}, Hkv={self.num_kv_heads}, D={self.model_dim}]")
+        if query.device != self.pool.device:
+            raise RuntimeError(f"the cache lies on {self.pool.device}; got a query on {query.device}")
+        if kv_start is not None and (kv_start.device != self.pool.device or kv_start.dtype != torch.int32 or kv_start.numel() < B
+                                     or not kv_start.is_contiguous()):
+            raise RuntimeError(f"kv_start is a contiguous int32 tensor [{B}] on {self.pool.device}; got {kv_start.dtype} "
+                               f"{tuple(kv_start.shape)} on {kv_start.device}")
         if attention_mask is not None:
             m = attention_mask
+            if m.device != self.pool.device:
+                raise RuntimeError(f"the cache lies on {self.pool.device}; got a mask on {m.device}")
             if m.dim() != 4 or m.size(1) != 1 or m.size(0) not in (1, B) or m.size(2) not in (1, S):
                 raise RuntimeError(f"paged attention takes a mask [B|1, 1, S|1, L]; got {tuple(m.shape)}")
             if m.dtype not in (torch.float32, torch.bfloat16):
