@@ -339,9 +339,10 @@ class PagedKVCache(KVCacheBase):
         head_step = h_in // self.num_kv_heads  # de-duplicate a repeat_kv-expanded input
         st = self.state
         lib = nat.load()
-        if (self._graph is not None and counts is None and (self.fuse_append or self.f32) and T <= 32
+        if (self._graph is not None and self._graph._recording and counts is None and (self.fuse_append or self.f32) and T <= 32
                 and self._pending is None and not self._graph_appended):
-            # a step of a decode graph: blocks and table were prepared for every step, and the lengths advance on the
+            # the step of a decode graph, on its eager run or under capture (run by itself later it ends the graph like
+            # any other operation, see _flush): blocks and table were prepared for every step, and the lengths advance on the
             # device.  The append rides in the attention launch; over an fp32 pool only with up to 32 query rows per KV
             # head (else, or with fuse_append off: a launch of its own, its positions taken from the graph's frozen
             # lengths plus the device counter).

@@ -55,6 +55,7 @@ class DecodeGraph:
             c._graph = self
         try:
             self._reserved = False
+            self._recording = True  # until the step is captured, the caches' appends and attention calls are the step's
             side = stream or torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
@@ -70,21 +71,22 @@ class DecodeGraph:
                 with torch.cuda.graph(self.graph, stream=side):
                     self.result = step_fn()
                     self.counter.add_(self.new_tokens)
-                self._capturing = False
+                self._capturing = self._recording = False
                 self._restore()
             torch.cuda.current_stream().wait_stream(side)
         except Exception:
             # a refused capture leaves the caches as they were: whatever the failed step appended is forgotten
-            self._capturing = False
+            self._capturing = self._recording = False
             self.close()
             self._restore()
             raise
 
-    _capturing = False
+    _capturing = _recording = False
 
     def _restore(self) -> None:
         for c, (lens, seq_len) in zip(self.caches, self._host):
             c.lens, c.seq_len, c._pending, c._graph_appended = lens.copy(), seq_len, None, False
+            c._query_rope = None
 
     def reserve(self, new_tokens: int) -> None:
         """Called by the first ``update_cache`` of the eager run: blocks and table for every future position."""
