@@ -83,6 +83,12 @@ constexpr uint32_t kMaskFloorBf16x2 = 0xf180f180u;  // the same value as a pair 
 // How far (in powers of two of the weight) a row's scores may rise above the softmax reference before the reference
 // is moved and the accumulators rescaled.
 constexpr float kLazyLog2 = 8.0f;
+// Where a row's reference lies beyond this, in powers of two of the weight, exponents are formed from the difference score -
+// reference, and every unit goes through the branch that does it (m_top = -inf).  Nearer, reference * c is subtracted inside one
+// multiply-add: rounded to 24 bits it is off by up to 2^-8 there, for all weights of the row alike.  Far out -- a mask filled
+// with -1e9 is at 2^30.4, one with -1e30 at 2^100.2 -- that rounding would be whole powers of two: weights overflow, or all
+// weights of the row vanish.  The floor itself is exact (see kMaskFloor).
+constexpr float kFarLog2 = 0x1p16f;
 
 __device__ __forceinline__ float xor_lanes(float v, int mask) { return __shfl_xor(v, mask, 64); }
 
@@ -444,6 +450,15 @@ __device__ __forceinline__ void softmax_and_output(const f32x4 (&sc)[NQT][2], co
       st.m[qt] = m_new;
       st.m_top[qt] = m_new + kLazyLog2 / c;
       st.m_neg[qt] = -(m_use * c);
+      if (HAS_MASK) {  // (see kFarLog2)
+        const bool far = fabsf(st.m_neg[qt]) > kFarLog2 && m_use != kMaskFloor;
+        st.m_top[qt] = far ? kNegInf : st.m_top[qt];
+        st.m_neg[qt] = far ? 0.f : st.m_neg[qt];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][i] -= far ? m_use : 0.f;
+      }
       st.l[qt] *= alpha;
 #pragma unroll
       for (int j = 0; j < MT; ++j) st.o[qt][j] *= alpha;

@@ -345,13 +345,6 @@ struct WalkRows {
 template <int BITS>
 constexpr float kWeightShift = BITS == 4 ? 7.f : 0.f;
 
-// Where a row's reference lies beyond this, in powers of two of the weight, exponents are formed from the difference score -
-// reference, and every unit goes through the branch that does it (m_top = -inf).  Nearer, reference * c is subtracted inside one
-// multiply-add: rounded to 24 bits it is off by up to 2^-8 there, for all weights of the row alike, and a weight stays below
-// 2^15.02.  Far out -- a mask filled with -1e9 is at 2^30.4 -- that rounding would be whole powers of two: halves overflow, or
-// all weights of the row vanish.
-constexpr float kFarLog2 = 0x1p16f;
-
 // Query row -> operand registers; 4-bit pools: as halves, times the power of two that brings the row's largest component to
 // [2^14, 2^15) (returned as its exponent; the four lanes (n, 0..3) of a row agree).
 template <int BITS, int D>
@@ -497,7 +490,7 @@ __device__ __forceinline__ void walk_weights(f32x4 (&sc)[NQT][2], WalkRows<D, NQ
       const float alpha = __builtin_amdgcn_exp2f((m_old - m_use) * c);
       st.m[qt] = m_new;
       const float neg = kWeightShift<BITS> - m_use * c;
-      const bool far = fabsf(neg) > kFarLog2 && m_use != kMaskFloor;  // (the floor is exact: see kMaskFloor)
+      const bool far = fabsf(neg) > kFarLog2 && m_use != kMaskFloor;  // (a weight of a near row stays below 2^15.02)
       st.m_top[qt] = far ? kNegInf : m_new + kLazyLog2 / c;
       st.m_neg[qt] = far ? kWeightShift<BITS> : neg;
 #pragma unroll
