@@ -325,10 +325,6 @@ class PagedKVCache(KVCacheBase):
             k, v = (torch.nn.functional.pad(t, (0, self.head_dim - self.model_dim)) for t in (k, v))
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise RuntimeError(f"the cache holds {self.dtype}; got {k.dtype} / {v.dtype}")
-        ks = k.stride()
-        per16 = 4 if self.f32 else 8  # elements in 16 bytes
-        if ks[3] != 1 or ks != v.stride() or ks[0] % per16 or ks[1] % per16 or ks[2] % per16:
-            k, v = k.contiguous(), v.contiguous()
         if (self.f32 or self.kv_bits == 4 or self.window) and rope is not None:
             # rotated in a launch of its own; the attention call that follows does the same with its queries
             _, k = rope(None, k)
@@ -336,6 +332,10 @@ class PagedKVCache(KVCacheBase):
             keep_query_rope = True
         else:
             keep_query_rope = False
+        ks = k.stride()  # (the keys' and the values': a rotation may have laid out the keys anew)
+        per16 = 4 if self.f32 else 8  # elements in 16 bytes
+        if ks[3] != 1 or ks != v.stride() or ks[0] % per16 or ks[1] % per16 or ks[2] % per16:
+            k, v = k.contiguous(), v.contiguous()
         head_step = h_in // self.num_kv_heads  # de-duplicate a repeat_kv-expanded input
         st = self.state
         lib = nat.load()
