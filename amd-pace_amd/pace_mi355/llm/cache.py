@@ -336,6 +336,8 @@ class PagedKVCache(KVCacheBase):
         per16 = 4 if self.f32 else 8  # elements in 16 bytes
         if ks[3] != 1 or ks != v.stride() or ks[0] % per16 or ks[1] % per16 or ks[2] % per16:
             k, v = k.contiguous(), v.contiguous()
+        if k.data_ptr() % 16 or v.data_ptr() % 16:
+            k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
         head_step = h_in // self.num_kv_heads  # de-duplicate a repeat_kv-expanded input
         st = self.state
         lib = nat.load()
@@ -604,9 +606,11 @@ class PagedKVCache(KVCacheBase):
             query, D = torch.nn.functional.pad(query, (0, self.head_dim - self.model_dim)), self.head_dim
         qs = query.stride()
         per16 = 4 if self.f32 else 8
-        if qs[3] != 1 or qs[0] % per16 or qs[1] % per16 or qs[2] % per16 or query.data_ptr() % 16:
+        if qs[3] != 1 or qs[0] % per16 or qs[1] % per16 or qs[2] % per16:
             query = query.contiguous()
-            qs = query.stride()
+        if query.data_ptr() % 16:
+            query = query.clone(memory_format=torch.contiguous_format)
+        qs = query.stride()
         if self.f32 and self._pending is not None and self._graph is None and S * (hq // self.num_kv_heads) > 32:
             self._flush()  # over an fp32 pool the append rides in launches of up to 32 query rows per KV head
         rope = self._query_rope  # (a call that is refused leaves it, and a held-back append, for the next one)

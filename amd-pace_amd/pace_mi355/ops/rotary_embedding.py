@@ -93,7 +93,7 @@ def _strided(x: torch.Tensor) -> torch.Tensor:
     step = 8 if x.dtype == torch.bfloat16 else 1  # bf16 rows move in 16-byte chunks
     ok = x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(
         s % step == 0 and (s > 0 or n == 1) for s, n in zip(x.stride()[:3], x.shape[:3]))
-    return x if ok else x.contiguous()
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
 def launch_rope_apply(desc: nat.RopeDesc, query: Optional[torch.Tensor], key: Optional[torch.Tensor],
