@@ -62,7 +62,8 @@ __device__ __forceinline__ _Float16 half_from(uint32_t b) { return __builtin_bit
 // Value e of a code dword as the number it is, -8 .. 7.
 __device__ __forceinline__ float q4_code(uint32_t w, int e) { return (float)((int)((w >> q4_bit(e)) & 15u) - 8); }
 
-// The eight codes of a dword as halves -8 .. 7, in element order.  `and-or` with the bits of 1024 makes a pair of halves 1024 +
+// The eight codes of a dword as halves -8 .. 7, in element order, by the published way of or-ing small integers into the mantissa of a
+// half of 1024 (Kim, Henry, Fahim, Awadalla, "Who Says Elephants Can't Run", 2022).  `and-or` with the bits of 1024 makes a pair of halves 1024 +
 // (code + 8) of the low nibbles and 1024 + 16 (code + 8) of the next ones; one packed add or multiply-add takes the
 // offset out again, exactly.  One shift per dword and 2 instructions per pair; `or_bits` comes from q4_or_bits().
 __device__ __forceinline__ void q4_codes(uint32_t w, uint32_t or_bits, f16x2 (&c)[4]) {
@@ -85,11 +86,12 @@ __device__ __forceinline__ uint32_t q4_or_bits() {
 // Quantises a group of 32 bf16 values held by four neighbouring lanes (eight each, lanes 4 k .. 4 k + 3, all active): the group's
 // step and middle, and this lane's codes (+ 8) as byte 2 of eight words.
 //
-// Codes are decided as by exact arithmetic.  y = x / s + (136 - m / s), one multiply-add with the reciprocal, lies in [128, 144): its
-// last place is 2^-16, and as |m / s| <= 64 (else the group takes the other way) it is off by less than one: 2^-17 each for
-// the added constant and for the sum, 9 * 2^-23 for the reciprocal.  Adding one half to the bits rounds it, the code is
-// then byte 2, and a fraction within two places of a border (6 values in 100 000) is decided again.
-// a - b == d + q4_rest(a, b, d) exactly, d the rounded difference.
+// Codes are decided as by arithmetic in double precision, in which the format is defined.  y = x / s + (136 - m / s), one
+// multiply-add with the reciprocal, lies in [128, 144): its last place is 2^-16, and as |m / s| <= 64 (else the group takes the
+// other way) it is off by less than one: 2^-17 each for the added constant and for the sum, 9 * 2^-23 for the reciprocal.  Adding
+// one half to the bits rounds it, the code is then byte 2, and a fraction within two places of a border (6 values in 100 000)
+// is decided again.
+// a - b == d + q4_rest(a, b, d) exactly, d the rounded difference (the error-free sum of two numbers: Knuth, Moller).
 __device__ __forceinline__ float q4_rest(float a, float b, float d) {
   const float back = d - a;
   return (a - (d - back)) - (b + back);

@@ -42,7 +42,7 @@ __device__ __forceinline__ int q4_v_dim(int r) {
 // covers only some of its eight tokens it is read, changed and written back.
 // 8 prompts of 4096 tokens, 8 heads of 128, stored (176 MB) and read back (the same): 79 us, 4.5 TB/s, where a plain copy moves
 // 5.1.  Two, four or eight blocks per workgroup with the next one's rows under way took 2, 3 and 6 us more: the workgroups
-// that share a compute unit hide the loads already.  One token each of 64 sequences, stored and read back: 10 us, latency.
+// that share a compute unit hide the loads already.  The store alone: 51 us, 3.5 TB/s.  One token each of 64 sequences, stored and read back: 10 us, latency.
 template <int D>
 __global__ __launch_bounds__(2 * D) void q4_append_paged_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
                                                                 const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh, int64_t st,
@@ -98,7 +98,9 @@ __global__ __launch_bounds__(2 * D) void q4_append_paged_kernel(pace_kv_pool_t p
 // By slot: 16 consecutive tokens of the input, wherever their slots lie.  Tokens of one V dword may then sit in two workgroups; a
 // dword not covered in full is changed by atomics on its own bits (each bit has one writer as long as no slot is named
 // twice, so the order does not matter).
-// 262144 tokens of 8 heads of 128 (1.4 GB): 490 us; 1135 us while every thread looked for the dwords token by token in LDS.
+// 262144 tokens of 8 heads of 128 (1.4 GB) in order: 481 to 492 us, 2.9 TB/s; by position the same takes 364.  What it costs more is
+// the V dwords, put together token by token although 16 tokens in order are two whole ones each; 1135 us while every thread
+// looked for the dwords token by token in LDS.  In shuffled order, a dword of V changed by two atomics per token: 1393 us.
 template <int D>
 __global__ __launch_bounds__(2 * D) void q4_append_slots_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
                                                                 const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh, int64_t st,

@@ -595,11 +595,14 @@ struct WalkTurns {
 // Groups of up to 16 query rows (decode; short appends, and prompts too short to fill the GPU otherwise): every wave walks units of
 // its own.  NW waves split a workgroup's units (wave w: units w, w + NW, ...), fetch one ahead, and merge through LDS.
 //
-// Bound: the pool's bytes.  64 sequences x 4096 tokens, 8 KV heads of 128 dims, 4 query heads each: 57 us for 336 MB of
-// 4-bit rows, 5.9 TB/s, where a plain read of as much reaches 6.0; 32 sequences through a window of 4096 tokens over a bf16
-// pool: 86 us, 6.3 TB/s (a window's rows partly come from the cache).  One sequence of 4096 tokens: 10.5 us, the latency of
-// two launches and of four units one after another.  Four waves and units in turn rather than one wave per run of units: a
-// workgroup's reads stay close together.  Two waves for 256 dims, whose state takes a wave's whole register file.
+// Bound: the pool's bytes.  64 sequences x 4096 tokens, 8 KV heads of 128 dims, 4 query heads each: 57 to 59 us for 336 MB of 4-bit
+// rows, over one pool or over four in turn, blocks in order or not (5.7 to 5.9 TB/s; a plain read of as much, four buffers in
+// turn: 5.5).  Behind a launch that has written half a gigabyte, whose lines are still on their way out of the cache, it
+// takes 79 us, and that plain read slows down from 65 to 109.  32 sequences through a window of 4096 tokens over a bf16 pool:
+// 83 to 85 us, 6.4 TB/s.  One sequence of 4096 tokens: 10.6 us, the latency of two launches and of four units one after
+// another.  Four waves and units in turn rather than one wave per run of units: a workgroup's reads stay close together.
+// Two waves for 256 dims, whose state takes a wave's whole register file and its accumulation registers (4 registers spill over
+// a 4-bit pool); 64 sequences x 2048, 16 heads of 256: 122 us, 5.5 TB/s.
 // Two or three row tiles per wave instead of walk_rows_kernel (36 rows): 123 us against 65 -- one wave per SIMD, and spills.
 // ---------------------------------------------------------------------------------
 template <int BITS, int D, bool HAS_MASK, int NW, int OCC>
@@ -740,13 +743,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
 // unpacking is paid once per workgroup; fetches run three units ahead of their use (two in registers, one in LDS), with
 // one barrier per unit.  A row's softmax state never leaves its wave.
 //
-// Bound: issue.  Matrix and vector instructions of the waves of one SIMD do not overlap, and per 32 tokens and tile 18 matrix
-// instructions (128 dims) stand next to some 60 vector ones (softmax, and a quarter of the unpacking).  4 sequences x 512 new
-// tokens over 4096 (8 KV heads of 128 dims, 4 query heads each): 170 us, 760 TFLOP/s, where a large fp16 matrix product
-// reaches 1200; the same with every wave unpacking for itself: 330 us.  32 sequences x 9 drafted tokens over 1000 .. 6000:
-// 65 us for 70 MB of rows, in which 36 of the 64 rows a workgroup computes are real.  Two tiles per wave above 64 rows halve
-// the LDS reads and the unpacking per row; with a mask tensor some registers spill at 128 dims, which costs less than twice as
-// many workgroups would.  Workgroups per compute unit under one tile, drafted tokens: 2 / 3 / 4 run 79 / 72 / 84 us.
+// Bound: issue for the larger part, waiting for the rest.  Matrix and vector instructions of the waves of one SIMD do not overlap;
+// by the counters they take, of a SIMD's cycles, 72 % (31 matrix, 42 vector) for 4 sequences x 512 new tokens over 4096 (8 KV
+// heads of 128 dims, 4 query heads each: 171 us, 755 TFLOP/s, where a large fp16 matrix product reaches 1294; with every wave
+// unpacking for itself 330 us), 51 % (13 and 38) for 32 sequences x 9 drafted tokens over 1000 .. 6000 (64 us, of which the
+// merge takes 12, for 118 MB of rows; 36 of the 64 rows a workgroup computes are real), and 57 % (25 and 31) for 2 x 1024
+// tokens through a window of 1024 over a bf16 pool (52 us).  The waves spend 20, 36 and 27 % of theirs at counter waits and
+// the barrier, so these launches have room left.  Two tiles per wave above 64 rows halve the LDS reads and the unpacking per
+// row.  Vector registers spilled with a mask tensor: 25 to 29 of two tiles and 15 to 17 of one at 128 dims, 7 or 8 at 256; every
+// form spills 31 to 98 scalar registers.  Workgroups per compute unit under one tile, drafted tokens: 2 / 3 / 4 run
+// 79 / 72 / 84 us.  With a mask tensor every unit up to the length is fetched and unpacked, also those that it leaves out for
+// all rows: a prompt of 4 x 2048 tokens takes 517 us with the models' causal mask and 201 without it.
 // ---------------------------------------------------------------------------------
 template <int BITS, int D, int NQT, bool HAS_MASK, int OCC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) void walk_rows_kernel(const WalkParams p) {
@@ -1046,7 +1053,11 @@ static WalkShape walk_shape_of(const pace_kv_pool_t* pool, const pace_paged_attn
   } else {
     // A workgroup per group lasts as long as the longest chain of units, or as a compute unit with its workgroups needs: under the causal
     // limit the groups of a fresh prompt have half as many units on average.  Sequences of long contexts may differ in
-    // length (only the bound is known here), which leaves compute units idle, unless there are many.
+    // length (only the bound is known here), which leaves compute units idle, unless there are many: up to 128 rows each, contexts
+    // of more than 160 units are taken for ragged.  The border lies between the sequences of 4096 tokens that were measured as
+    // equal and those of 1000 .. 6000 and 500 .. 8000 that were measured as ragged, and is a guess between them.  It costs equal
+    // long sequences the second launch (shared / not, us: 32 x 8000 65 to 70 / 60, 64 x 8000 114 / 107, 128 x 6000 169 / 160, 64 x 6000
+    // with 5 tokens 174 / 152) for what it saves ragged ones (64 x 500 .. 8000 57 / 74, 32 x 1000 .. 6000 with 9 tokens 62 / 145).
     const double fresh = a->causal && a->window == 0 ? std::min(a->q_len, a->max_seq_len) / (double)std::max(a->max_seq_len, 1) : 0.0;
     const double average = (double)units * (1.0 - 0.5 * fresh);
     const double ragged = rows <= 128 && a->batch > 1 && units > 160 ? 1.4 : 1.0;

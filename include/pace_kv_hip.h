@@ -38,19 +38,20 @@
  * fp32 too; the attention needs no work list, and a workspace only helps it when
  * the batch leaves compute units idle: with room for batch * num_q_heads * q_len
  * * parts * (head_dim + 4) floats it cuts every sequence over up to parts <= 64
- * workgroups); what folds other steps into
- * a launch (pace_rope_append_paged, args->rope, args->k_new) is bf16 only and
- * says so when handed such a pool.
+ * workgroups; args->k_new rides in launches of up to 32 query rows per KV head);
+ * what folds a rotation into a launch (pace_rope_append_paged, args->rope) is
+ * bf16 only and says so when handed such a pool.
  *
  * A pool may hold its rows in 4 bits (elem_bytes = PACE_KV_ELEM_Q4).  A row is
  * cut into groups of 32 dims; a group holds a step s and a middle m (halves)
  * and a code -8 .. 7 per value, and stands for s * code + m:
  *   s = the least half with 15 s >= max - min,  m = half(min + 8 s),
- *   code = round-half-even((x - m) / s) held in -8 .. 7 (0 where s = 0);
- * NaN counts as 0 and values are held at +-32768 before that.  Slabs take
- * 10 * head_dim bytes each for K and for V, head_dim as for bf16, strides in
- * BYTES (multiples of 16).  New tokens, gathered rows, queries and outputs are
- * bf16: append / append_paged / append_paged_at quantise, gather /
+ *   code = round-half-even((x - m) / s) held in -8 .. 7 (0 where s = 0),
+ * decided in double precision: what x - m loses there, below 2^-54 of it, does
+ * not break a tie.  NaN counts as 0 and values are held at +-32768 before that.
+ * Slabs take 10 * head_dim bytes each for K and for V, head_dim as for bf16,
+ * strides in BYTES (multiples of 16).  New tokens, gathered rows, queries and
+ * outputs are bf16: append / append_paged / append_paged_at quantise, gather /
  * gather_packed / gather_live read back, copy_blocks and compact_blocks move
  * the slabs as they are, and the attention entry points read the codes in place
  * (a fused append, args->k_new, is quantised first; no rotary embedding inside
