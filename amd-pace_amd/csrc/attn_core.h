@@ -454,10 +454,12 @@ __device__ __forceinline__ void softmax_and_output(const f32x4 (&sc)[NQT][2], co
         const bool far = fabsf(st.m_neg[qt]) > kFarLog2 && m_use != kMaskFloor;
         st.m_top[qt] = far ? kNegInf : st.m_top[qt];
         st.m_neg[qt] = far ? 0.f : st.m_neg[qt];
+        if (__any(far)) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][i] -= far ? m_use : 0.f;
+            for (int i = 0; i < 4; ++i) s[t][i] -= far ? m_use : 0.f;
+        }
       }
       st.l[qt] *= alpha;
 #pragma unroll
