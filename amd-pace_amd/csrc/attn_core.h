@@ -234,7 +234,7 @@ __device__ __forceinline__ void load_mask_regs(MaskRegs<NQT>& mr, const PagedAtt
 
 // The same values as fetched, for a caller that fetches a unit ahead: converting them where they are loaded would
 // make the wave wait for the load there.  bf16: eight values in w[qt][0]; fp32: in w[qt][0], w[qt][1].  Columns the mask
-// does not have come as -inf.
+// does not have come as -inf, which the conversion holds at the floor like any other: the caller leaves them out by their place.
 template <int NQT>
 struct MaskRaw {
   u32x4 w[NQT][2];

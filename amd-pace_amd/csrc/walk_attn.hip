@@ -39,10 +39,18 @@ struct Walk {
   __device__ __forceinline__ int unit(int i) const { return i < n_sink ? su0 + i : wu0 + (i - n_sink); }
 };
 
+// One past the last token that a row of query token s reads: the causal limit, the sequence's end, the mask's last column.
+template <bool HAS_MASK>
+__device__ __forceinline__ int walk_end(const WalkParams& p, int len, int s) {
+  const int end = HAS_MASK ? min(len, p.mask_len) : len;
+  return p.causal ? min(end, len - p.q_len + s + 1) : end;
+}
+
 // s_first, s_last: query tokens of the group's first and last row.
+template <bool HAS_MASK>
 __device__ __forceinline__ Walk walk_of(const WalkParams& p, int len, int start, int s_first, int s_last) {
   Walk w;
-  const int end = p.causal ? min(len, len - p.q_len + s_last + 1) : len;
+  const int end = walk_end<HAS_MASK>(p, len, s_last);
   int low = start;
   w.sink_end = start;
   if (p.window > 0) {
@@ -52,7 +60,9 @@ __device__ __forceinline__ Walk walk_of(const WalkParams& p, int len, int start,
   w.wu0 = low / 32;
   const int wu1 = end > low ? (end + 31) / 32 : w.wu0;
   w.su0 = start / 32;
-  w.n_sink = min(w.sink_end, end) > start ? max(min((min(w.sink_end, end) + 31) / 32, w.wu0) - w.su0, 0) : 0;
+  // (the sinks' last unit may be the window's first, unless the window is empty: a mask may end below it)
+  const int sinks = min(w.sink_end, end), su1 = end > low ? min((sinks + 31) / 32, w.wu0) : (sinks + 31) / 32;
+  w.n_sink = sinks > start ? max(su1 - w.su0, 0) : 0;
   w.total = w.n_sink + wu1 - w.wu0;
   return w;
 }
@@ -68,6 +78,7 @@ struct Group {
   int b, r_first, r_last, s_first, s_last, len, start;
   Walk walk;
 };
+template <bool HAS_MASK>
 __device__ __forceinline__ Group walk_group(const WalkParams& p, int j) {
   Group x;
   x.b = j / p.n_qgroups;
@@ -75,7 +86,7 @@ __device__ __forceinline__ Group walk_group(const WalkParams& p, int j) {
   x.r_first = qg * p.group_rows, x.r_last = min(p.q_len * p.n_rep, x.r_first + p.group_rows) - 1;
   x.s_first = x.r_first / p.n_rep, x.s_last = x.r_last / p.n_rep;
   x.len = walk_len(p, x.b), x.start = walk_start(p, x.b, x.len);
-  x.walk = walk_of(p, x.len, x.start, x.s_first, x.s_last);
+  x.walk = walk_of<HAS_MASK>(p, x.len, x.start, x.s_first, x.s_last);
   return x;
 }
 
@@ -91,22 +102,25 @@ __device__ __forceinline__ int wave_sum(int v) {
   for (int o = 1; o < 64; o *= 2) v += __shfl_xor(v, o, 64);
   return __builtin_amdgcn_readfirstlane(v);
 }
-__device__ __forceinline__ int group_units(const WalkParams& p, int j) { return j < p.batch * p.n_qgroups ? walk_group(p, j).walk.total : 0; }
+template <bool HAS_MASK>
+__device__ __forceinline__ int group_units(const WalkParams& p, int j) { return j < p.batch * p.n_qgroups ? walk_group<HAS_MASK>(p, j).walk.total : 0; }
+template <bool HAS_MASK>
 __device__ __forceinline__ Shares walk_shares(const WalkParams& p, int lane) {
   const int n = p.batch * p.n_qgroups;
   int mine = 0;
 #pragma unroll 4
-  for (int j = lane; j < n; j += 64) mine += group_units(p, j);
+  for (int j = lane; j < n; j += 64) mine += group_units<HAS_MASK>(p, j);
   Shares s;
   s.total = wave_sum(mine);
   s.share = walk_share(p, s.total);
   return s;
 }
 // The group that unit `at` of the run (at < total) lies in, and its place there.
+template <bool HAS_MASK>
 __device__ __forceinline__ void walk_find(const WalkParams& p, int at, int lane, int& j, int& off) {
   int before = 0;
   for (int base = 0;; base += 64) {
-    const int units = group_units(p, base + lane);
+    const int units = group_units<HAS_MASK>(p, base + lane);
     int upto = units;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
@@ -381,7 +395,7 @@ __device__ __forceinline__ int walk_row(const WalkParams& p, WalkRows<D, NQT>& s
   const bool valid = r < S * p.n_rep;
   const int s = valid ? r / p.n_rep : 0, hq = kvh * p.n_rep + (valid ? r % p.n_rep : 0), pos = len - S + s;
   st.s[qt] = s, st.hq[qt] = hq;
-  st.limit[qt] = valid ? (p.causal ? pos : len - 1) : -1;
+  st.limit[qt] = valid ? walk_end<HAS_MASK>(p, len, s) - 1 : -1;
   st.low[qt] = p.window > 0 ? pos - p.window + 1 : 0;
   const uint16_t* qp = p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh + (int64_t)s * p.q_ss + 8 * g;
 #pragma unroll
@@ -560,6 +574,7 @@ __device__ __forceinline__ void walk_store(const WalkParams& p, const WalkRows<D
 }
 
 // The pieces of groups that a workgroup works on, one after the other (wave-uniform): for (WalkTurns t(...); t.more(); t.next()).
+template <bool HAS_MASK>
 struct WalkTurns {
   const WalkParams& p;
   int kvh, w, j, off, left;
@@ -574,11 +589,11 @@ struct WalkTurns {
       off = w * p.part_units, left = w == p.shares - 1 ? 1 << 30 : p.part_units;  // (the last one: whatever there is)
       return;
     }
-    const Shares s = walk_shares(p, lane);
+    const Shares s = walk_shares<HAS_MASK>(p, lane);
     const int64_t at = (int64_t)w * s.share;
     if (at >= s.total) return;
     left = min(s.share, s.total - (int)at);
-    walk_find(p, (int)at, lane, j, off);
+    walk_find<HAS_MASK>(p, (int)at, lane, j, off);
   }
   // Units [begin, end) of group `x`; slot: where a partial result goes, -1: the group is covered in whole.
   __device__ __forceinline__ bool piece(const Group& x, int& begin, int& end, int& slot) {
@@ -611,7 +626,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
   __shared__ float merge_buf[(NW / 2) * SLOT_F];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  WalkTurns turns(p, lane);
+  WalkTurns<HAS_MASK> turns(p, lane);
   const int kvh = turns.kvh, S = p.q_len, R = S * p.n_rep, n_groups = p.batch * p.n_qgroups;
   // One sequence without a window and padding: its units do not depend on its length, and the first block ids are asked for
   // along with that.
@@ -622,7 +637,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     early = t < p.table_stride ? p.table[t] : 0;
   }
   do {
-    const Group x = walk_group(p, turns.j);
+    const Group x = walk_group<HAS_MASK>(p, turns.j);
     const int b = x.b, len = x.len, start = x.start;
     const Walk walk = x.walk;
     int i_begin, i_end, slot;
@@ -659,7 +674,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
     min_limit = __builtin_amdgcn_readfirstlane(min_limit);
     const int row_low = p.window > 0 ? len - S + x.s_first - p.window + 1 : 0;  // the first row's window, and the last row's
     const int max_low = p.window > 0 ? len - S + x.s_last - p.window + 1 : 0;
-    const int row_end = p.causal ? min(len, len - S + x.s_last + 1) : len;
+    const int row_end = walk_end<HAS_MASK>(p, len, x.s_last);
 
     auto take = [&](WalkUnit<BITS, D>& u, const MaskRaw<1>& m, int k) {
       const int t0 = 32 * walk.unit(i_begin + wave + NW * k);
@@ -751,7 +766,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, 8)
 // tokens through a window of 1024 over a bf16 pool (52 us).  The waves spend 20, 36 and 27 % of theirs at counter waits and
 // the barrier, so these launches have room left.  Two tiles per wave above 64 rows halve the LDS reads and the unpacking per
 // row.  Vector registers spilled with a mask tensor: 25 to 29 of two tiles and 15 to 17 of one at 128 dims, 7 or 8 at 256; every
-// form spills 31 to 98 scalar registers.  Workgroups per compute unit under one tile, drafted tokens: 2 / 3 / 4 run
+// form spills 29 to 100 scalar registers.  Workgroups per compute unit under one tile, drafted tokens: 2 / 3 / 4 run
 // 79 / 72 / 84 us.  With a mask tensor every unit up to the length is fetched and unpacked, also those that it leaves out for
 // all rows: a prompt of 4 x 2048 tokens takes 517 us with the models' causal mask and 201 without it.
 // ---------------------------------------------------------------------------------
@@ -761,10 +776,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
   __shared__ __attribute__((aligned(16))) u32x4 stage[2][OPERANDS * 64];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  WalkTurns turns(p, lane);
+  WalkTurns<HAS_MASK> turns(p, lane);
   const int kvh = turns.kvh, S = p.q_len, R = S * p.n_rep, n_groups = p.batch * p.n_qgroups;
   do {
-    const Group x = walk_group(p, turns.j);
+    const Group x = walk_group<HAS_MASK>(p, turns.j);
     const int b = x.b, len = x.len, start = x.start, r_first = x.r_first;
     const Walk walk = x.walk;
     int i_begin, i_end, slot;
@@ -772,7 +787,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
     ++turns.j;
     if (!some) continue;  // uniform over the workgroup
     const int wg_low = p.window > 0 ? len - S + x.s_first - p.window + 1 : 0;  // what no row of the workgroup reads (see walk_keep)
-    const int wg_end = p.causal ? min(len, len - S + x.s_last + 1) : len;
+    const int wg_end = walk_end<HAS_MASK>(p, len, x.s_last);
 
     const int32_t* row = p.table + (int64_t)b * p.table_stride;
     // Pool blocks of 64 units from c0 on, one per lane in each of two registers; never outside the pool.
@@ -813,7 +828,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, 8))) v
     min_limit = __builtin_amdgcn_readfirstlane(min_limit);
     const int row_low = p.window > 0 ? len - S + w_first / p.n_rep - p.window + 1 : 0;
     const int max_low = p.window > 0 ? len - S + w_last / p.n_rep - p.window + 1 : 0;
-    const int row_end = !any_rows ? 0 : (p.causal ? min(len, len - S + w_last / p.n_rep + 1) : len);
+    const int row_end = any_rows ? walk_end<HAS_MASK>(p, len, w_last / p.n_rep) : 0;
 
     // One turn: unit i + 1 of the set goes from `next` into LDS, `next` fetches unit i + 3, unit i is used.  With two tiles per wave LDS
     // reads travel behind vector work: the K operands are asked for before the unpacking, the V operands before the softmax
@@ -901,14 +916,14 @@ __global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int
   if (row0 >= total_rows) return;  // (WPR == 1 only: whole waves)
   const int S = p.q_len, n_groups = p.batch * p.n_qgroups;
   const bool one_group = p.part_units > 0 && n_groups == 1;
-  int mine, share;  // units of the first 64 groups, one per lane
+  int mine, share;  // units of the first 64 groups, one per lane  (without a mask its length is past every sequence's)
   if (one_group) {
-    mine = group_units(p, 0), share = p.part_units;
+    mine = group_units<true>(p, 0), share = p.part_units;
   } else {
-    mine = group_units(p, lane);
+    mine = group_units<true>(p, lane);
     int total = mine;
 #pragma unroll 4
-    for (int i = lane + 64; i < n_groups; i += 64) total += group_units(p, i);
+    for (int i = lane + 64; i < n_groups; i += 64) total += group_units<true>(p, i);
     share = walk_share(p, wave_sum(total));
   }
   int last_j = -1, w0 = 0, n_parts = 0, late = 0;
@@ -918,9 +933,9 @@ __global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int
     const int j = b * p.n_qgroups + p.n_qgroups - 1 - qg;
     if (j != last_j) {  // the group's units, and where they begin in the run of all units
       int before = lane < j ? mine : 0;
-      for (int i = lane + 64; i < j; i += 64) before += group_units(p, i);
+      for (int i = lane + 64; i < j; i += 64) before += group_units<true>(p, i);
       const int at = one_group ? 0 : wave_sum(before);
-      const int units = j < 64 ? __builtin_amdgcn_readlane(mine, j) : group_units(p, j);
+      const int units = j < 64 ? __builtin_amdgcn_readlane(mine, j) : group_units<true>(p, j);
       w0 = at / share, n_parts = units > 0 ? min((at + units - 1) / share, p.shares - 1) - w0 + 1 : 0;
       late = at % share != 0 ? 1 : 0;
       last_j = j;
@@ -1152,7 +1167,7 @@ int launch_walk(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* a, con
   p.num_blocks = pool->num_blocks, p.num_kv_heads = pool->num_kv_heads;
   p.table = a->block_table, p.table_stride = a->table_stride;
   p.seq_lens = a->seq_lens, p.len_bias = a->seq_len_bias, p.len_bias_dev = a->seq_len_bias_ptr, p.kv_start = a->kv_start;
-  p.mask = a->mask, p.mask_is_f32 = a->mask_dtype == PACE_DTYPE_F32, p.mask_len = a->mask_len;
+  p.mask = a->mask, p.mask_is_f32 = a->mask_dtype == PACE_DTYPE_F32, p.mask_len = a->mask ? a->mask_len : 0x7fffffff;
   p.m_sb = a->mask_stride_b, p.m_ss = a->mask_stride_s;
   p.n_rep = a->num_q_heads / pool->num_kv_heads, p.q_len = a->q_len, p.num_q_heads = a->num_q_heads, p.batch = a->batch;
   p.causal = a->causal;
