@@ -62,10 +62,10 @@ __device__ __forceinline__ _Float16 half_from(uint32_t b) { return __builtin_bit
 // Value e of a code dword as the number it is, -8 .. 7.
 __device__ __forceinline__ float q4_code(uint32_t w, int e) { return (float)((int)((w >> q4_bit(e)) & 15u) - 8); }
 
-// The eight codes of a dword as halves -8 .. 7, in element order, by the published way of or-ing small integers into the mantissa of a
-// half of 1024 (Kim, Henry, Fahim, Awadalla, "Who Says Elephants Can't Run", 2022).  `and-or` with the bits of 1024 makes a pair of halves 1024 +
-// (code + 8) of the low nibbles and 1024 + 16 (code + 8) of the next ones; one packed add or multiply-add takes the
-// offset out again, exactly.  One shift per dword and 2 instructions per pair; `or_bits` comes from q4_or_bits().
+// The eight codes of a dword as halves -8 .. 7, in element order, by the published way of or-ing small integers into the mantissa
+// of a half of 1024 (Kim, Henry, Fahim, Awadalla, "Who Says Elephants Can't Run", 2022).  `and-or` with the bits of 1024 makes
+// a pair of halves 1024 + (code + 8) of the low nibbles and 1024 + 16 (code + 8) of the next ones; one packed add or
+// multiply-add takes the offset out again, exactly.  One shift per dword and 2 instructions per pair; `or_bits` comes from q4_or_bits().
 __device__ __forceinline__ void q4_codes(uint32_t w, uint32_t or_bits, f16x2 (&c)[4]) {
   const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
 #pragma unroll

@@ -42,7 +42,8 @@ __device__ __forceinline__ int q4_v_dim(int r) {
 // covers only some of its eight tokens it is read, changed and written back.
 // 8 prompts of 4096 tokens, 8 heads of 128, stored (176 MB) and read back (the same): 79 us, 4.5 TB/s, where a plain copy moves
 // 5.1.  Two, four or eight blocks per workgroup with the next one's rows under way took 2, 3 and 6 us more: the workgroups
-// that share a compute unit hide the loads already.  The store alone: 51 us, 3.5 TB/s.  One token each of 64 sequences, stored and read back: 10 us, latency.
+// that share a compute unit hide the loads already.  The store alone: 51 us, 3.5 TB/s.  One token each of 64 sequences,
+// stored and read back: 10 us, latency.
 template <int D>
 __global__ __launch_bounds__(2 * D) void q4_append_paged_kernel(pace_kv_pool_t pool, const uint16_t* __restrict__ k_new,
                                                                 const uint16_t* __restrict__ v_new, int64_t sb, int64_t sh, int64_t st,

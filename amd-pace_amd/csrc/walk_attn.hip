@@ -916,7 +916,7 @@ __global__ __launch_bounds__(256) void walk_merge_kernel(const WalkParams p, int
   if (row0 >= total_rows) return;  // (WPR == 1 only: whole waves)
   const int S = p.q_len, n_groups = p.batch * p.n_qgroups;
   const bool one_group = p.part_units > 0 && n_groups == 1;
-  int mine, share;  // units of the first 64 groups, one per lane  (without a mask its length is past every sequence's)
+  int mine, share;  // units of the first 64 groups, one per lane (<true>: without a mask its length is past every sequence's)
   if (one_group) {
     mine = group_units<true>(p, 0), share = p.part_units;
   } else {

@@ -439,7 +439,8 @@ size_t pace_paged_attn_workspace_bytes(int32_t batch, int32_t num_q_heads, int32
 
 /* The same for one particular call: the scratch pace_paged_attn_decode / _verify use for this pool and these arguments
  * (whose workspace fields are not read).  Over a 4-bit pool or through a window less is accepted, and none at all:
- * the context is then cut over fewer workgroups.  0 also for arguments that the launch refuses. */
+ * the context is then cut over fewer workgroups.  0 also for a partition_tokens that the launch
+ * refuses. */
 size_t pace_paged_attn_workspace_for(const pace_kv_pool_t* pool, const pace_paged_attn_args_t* args);
 
 size_t pace_paged_attn_workspace_bytes_for_parts(int32_t batch, int32_t num_q_heads, int32_t q_len,
